@@ -13,6 +13,8 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 CML_Q4_0, CML_Q8_0, CML_Q4_K, CML_Q6_K = 2, 8, 12, 14
+CML_F32, CML_F16, CML_BF16 = 0, 1, 30  # value types of the int8 lane and of scoring
+CML_ROUTE_SOFTMAX, CML_ROUTE_SIGMOID = 0, 1
 FORMATS = {"Q4_0": CML_Q4_0, "Q8_0": CML_Q8_0, "Q4_K": CML_Q4_K, "Q6_K": CML_Q6_K}
 
 EXPORTS = [
@@ -27,6 +29,8 @@ EXPORTS = [
     "cml_gemv", "cml_gemm", "cml_block_dots", "cml_matmul_workspace_bytes", "cml_matmul_f32", "cml_matmul_f32_pair", "cml_matmul_f32_multi", "cml_matmul_f32_static",
     "cml_moe_route_top_k", "cml_moe_route_softmax_top_k", "cml_moe_workspace_bytes", "cml_moe_ffn", "cml_moe_ffn_ex", "cml_moe_ffn_logits",
     "cml_moe_plan", "cml_moe_gemv_routed", "cml_moe_weighted_sum",
+    "cml_add_rms_norm_i8", "cml_quantize_i8", "cml_dequantize_i8", "cml_matmul_i8", "cml_moe_route_scored",
+    "cml_token_log_probs_workspace_bytes", "cml_token_log_probs",
     "cml_quantize_weights_host", "cml_try_linear_rows", "cml_try_q8_0_block_linear_row",
 ]
 
@@ -121,6 +125,15 @@ def lib() -> C.CDLL:
     L.cml_moe_gemv_routed.argtypes = [vp, i32, vp, vp, vp, vp, vp, i32, i64, vp, vp]
     L.cml_moe_weighted_sum.argtypes = [vp, vp, vp, i64, i32, i64, vp, vp]
     L.cml_glu_quantize.argtypes = [i32, i32, vp, vp, i64, i64, vp, vp, vp]
+    f32 = C.c_float
+    L.cml_add_rms_norm_i8.argtypes = [i32, vp, i64, vp, i64, vp, f32, i64, i64, vp, i64, vp, vp, i64, vp, vp]
+    L.cml_quantize_i8.argtypes = [i32, vp, i64, i64, i64, vp, i64, vp, vp]
+    L.cml_dequantize_i8.argtypes = [vp, i64, vp, i64, i64, i32, vp, i64, vp]
+    L.cml_matmul_i8.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, vp, i32, vp, i64, vp]
+    L.cml_moe_route_scored.argtypes = [i32, i32, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp]
+    L.cml_token_log_probs_workspace_bytes.argtypes = [i64, i64, i32]
+    L.cml_token_log_probs_workspace_bytes.restype = sz
+    L.cml_token_log_probs.argtypes = [i32, vp, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp, vp, sz, vp]
     L.cml_quantize_weights_host.argtypes = [i32, vp, sz, vp, i32]
     L.cml_try_linear_rows.argtypes = [i32, vp, vp, vp, sz, i64, i64, i64, vp]
     L.cml_try_q8_0_block_linear_row.argtypes = [vp, vp, vp, sz, i64, i64, vp]

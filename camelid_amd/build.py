@@ -26,6 +26,7 @@ SOURCES = [
     "gemv_q8q4.hip",
     "gemv_q6k.hip",
     "moe.hip",
+    "int8_rows.hip", "matmul_i8.hip", "moe_route.hip", "token_log_probs.hip",
     "weight_quantize.cpp",
 ]
 

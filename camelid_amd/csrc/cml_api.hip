@@ -716,6 +716,143 @@ int cml_argmax_f32(const float *logits_dev, int64_t n_rows, int64_t n, uint32_t 
     return launch_argmax_f32(logits_dev, n_rows, n, out_idx_dev, as_stream(stream));
 }
 
+// ---- the int8 lane and scoring -----------------------------------------------------------------------
+
+// A row-major operand of element size `bytes`: null, off its element's boundary, or rows that overlap.
+static int bad_rows(const char *what, const void *p, int64_t stride, int64_t cols, int64_t n_rows, int bytes) {
+    if (!p) return fail(CML_ERR_INVALID, "null %s", what);
+    if (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) != 0) return fail(CML_ERR_INVALID, "%s is not aligned to its elements", what);
+    if (stride < cols && n_rows > 1) return fail(CML_ERR_SHAPE, "rows of %s are %lld elements apart and hold %lld", what, (long long)stride, (long long)cols);
+    return CML_OK;
+}
+static int bad_f32(const char *what, const void *p) {
+    if (!p) return fail(CML_ERR_INVALID, "null %s", what);
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(CML_ERR_INVALID, "%s is not 4-byte aligned", what);
+    return CML_OK;
+}
+constexpr int64_t kMostI8Row = 65536;      // values of a row that the quantizing kernels hold in registers
+constexpr int64_t kMostI8Cols = 131071;    // |sum| <= 2^14 * cols stays below 2^31
+constexpr int64_t kMostRows = 1 << 30;     // rows or tokens of one call: a grid's workgroups are counted in 31 bits
+
+int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const void *residual_dev, int64_t residual_stride, const float *weight_dev, float eps, int64_t n_tokens,
+                        int64_t cols, void *sum_dev, int64_t sum_stride, float *normed_dev, int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream) {
+    if (int rc = check_ready()) return rc;
+    if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
+    if (n_tokens < 0 || cols < 0 || n_tokens > kMostRows) return fail(CML_ERR_SHAPE, "%lld rows of %lld values", (long long)n_tokens, (long long)cols);
+    if (n_tokens == 0 || cols == 0) return CML_OK;
+    if (cols > kMostI8Row) return fail(CML_ERR_UNSUPPORTED, "a row of %lld values: at most %lld", (long long)cols, (long long)kMostI8Row);
+    const int bytes = type_bytes(dtype);
+    if (int rc = bad_rows("x", x_dev, x_stride, cols, n_tokens, bytes)) return rc;
+    if (residual_dev)
+        if (int rc = bad_rows("residual", residual_dev, residual_stride, cols, n_tokens, bytes)) return rc;
+    if (sum_dev)
+        if (int rc = bad_rows("sum", sum_dev, sum_stride, cols, n_tokens, bytes)) return rc;
+    if (int rc = bad_rows("q", q_dev, q_stride, cols, n_tokens, 1)) return rc;
+    if (int rc = bad_f32("weight", weight_dev)) return rc;
+    if (int rc = bad_f32("scales", scales_dev)) return rc;
+    if (normed_dev)
+        if (int rc = bad_f32("normed", normed_dev)) return rc;
+    return launch_add_rms_norm_i8(dtype, x_dev, x_stride, residual_dev, residual_stride, weight_dev, eps, n_tokens, cols, sum_dev, sum_stride, normed_dev, q_dev, q_stride, scales_dev,
+                                  as_stream(stream));
+}
+
+int cml_quantize_i8(int dtype, const void *x_dev, int64_t x_stride, int64_t n_rows, int64_t cols, int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream) {
+    if (int rc = check_ready()) return rc;
+    if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
+    if (n_rows < 0 || cols < 0 || n_rows > kMostRows) return fail(CML_ERR_SHAPE, "%lld rows of %lld values", (long long)n_rows, (long long)cols);
+    if (n_rows == 0 || cols == 0) return CML_OK;
+    if (cols > kMostI8Row) return fail(CML_ERR_UNSUPPORTED, "a row of %lld values: at most %lld", (long long)cols, (long long)kMostI8Row);
+    if (int rc = bad_rows("x", x_dev, x_stride, cols, n_rows, type_bytes(dtype))) return rc;
+    if (int rc = bad_rows("q", q_dev, q_stride, cols, n_rows, 1)) return rc;
+    if (int rc = bad_f32("scales", scales_dev)) return rc;
+    return launch_quantize_i8(dtype, x_dev, x_stride, n_rows, cols, q_dev, q_stride, scales_dev, as_stream(stream));
+}
+
+int cml_dequantize_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev, int64_t n_rows, int64_t cols, int dtype, void *out_dev, int64_t out_stride, cml_stream_t stream) {
+    if (int rc = check_ready()) return rc;
+    if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
+    if (n_rows < 0 || cols < 0 || cols > kMostRows || (cols > 0 && n_rows > kMostRows / ((cols + 4095) / 4096))) return fail(CML_ERR_SHAPE, "%lld rows of %lld values", (long long)n_rows, (long long)cols);
+    if (n_rows == 0 || cols == 0) return CML_OK;
+    if (int rc = bad_rows("q", q_dev, q_stride, cols, n_rows, 1)) return rc;
+    if (int rc = bad_rows("out", out_dev, out_stride, cols, n_rows, type_bytes(dtype))) return rc;
+    if (int rc = bad_f32("scales", scales_dev)) return rc;
+    return launch_dequantize_i8(q_dev, q_stride, scales_dev, n_rows, cols, dtype, out_dev, out_stride, as_stream(stream));
+}
+
+int cml_matmul_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev, int64_t n_tokens, const int8_t *w_dev, int64_t w_stride, const float *w_scales_dev, int64_t rows, int64_t cols,
+                  const float *bias_dev, int dtype, void *out_dev, int64_t out_stride, cml_stream_t stream) {
+    if (int rc = check_ready()) return rc;
+    if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
+    if (n_tokens < 0 || rows < 0 || cols <= 0 || cols > kMostI8Cols) return fail(CML_ERR_SHAPE, "%lld tokens, %lld rows of %lld values (1 to %lld)", (long long)n_tokens, (long long)rows, (long long)cols, (long long)kMostI8Cols);
+    if (n_tokens > (1 << 20) || rows > (1 << 27)) return fail(CML_ERR_UNSUPPORTED, "%lld tokens and %lld rows in one call", (long long)n_tokens, (long long)rows);
+    if (n_tokens == 0 || rows == 0) return CML_OK;
+    if (int rc = bad_rows("q", q_dev, q_stride, cols, n_tokens, 1)) return rc;
+    if (int rc = bad_rows("w", w_dev, w_stride, cols, rows, 1)) return rc;
+    if (int rc = bad_rows("out", out_dev, out_stride, rows, n_tokens, type_bytes(dtype))) return rc;
+    if (int rc = bad_f32("scales", scales_dev)) return rc;
+    if (int rc = bad_f32("w_scales", w_scales_dev)) return rc;
+    if (bias_dev)
+        if (int rc = bad_f32("bias", bias_dev)) return rc;
+    const int rc = launch_matmul_i8(q_dev, q_stride, scales_dev, n_tokens, w_dev, w_stride, w_scales_dev, rows, cols, bias_dev, dtype, out_dev, out_stride, as_stream(stream));
+    if (rc == CML_OK) g_runs.fetch_add(1, std::memory_order_relaxed);
+    return rc;
+}
+
+int cml_moe_route_scored(int score, int dtype, const void *logits_dev, int64_t logits_stride, const float *bias_dev, int64_t n_tokens, int n_experts, int n_groups, int groups_kept, int group_top,
+                         int k, int renormalise, float weight_scale, int32_t *idx_dev, float *weight_dev, cml_stream_t stream) {
+    if (int rc = check_ready()) return rc;
+    if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
+    if (score != CML_ROUTE_SOFTMAX && score != CML_ROUTE_SIGMOID) return fail(CML_ERR_INVALID, "unknown score %d", score);
+    if (n_tokens < 0 || n_tokens > kMostRows || n_experts < 1 || n_experts > 1024) return fail(CML_ERR_SHAPE, "%lld tokens, %d experts (1 to 1024)", (long long)n_tokens, n_experts);
+    if (n_groups < 1 || n_groups > 64 || n_experts % n_groups != 0) return fail(CML_ERR_SHAPE, "%d experts in %d groups (1 to 64, of one size)", n_experts, n_groups);
+    if (groups_kept < 1 || groups_kept > n_groups || group_top < 1 || group_top > 2) return fail(CML_ERR_SHAPE, "%d of %d groups kept, by their %d best", groups_kept, n_groups, group_top);
+    if (k < 1 || k > 64 || k > groups_kept * (n_experts / n_groups)) return fail(CML_ERR_SHAPE, "%d experts of %d (1 to 64)", k, groups_kept * (n_experts / n_groups));
+    if (n_tokens == 0) return CML_OK;
+    if (int rc = bad_rows("logits", logits_dev, logits_stride, n_experts, n_tokens, type_bytes(dtype))) return rc;
+    if (bias_dev)
+        if (int rc = bad_f32("bias", bias_dev)) return rc;
+    if (int rc = bad_f32("idx", idx_dev)) return rc;
+    if (int rc = bad_f32("weight", weight_dev)) return rc;
+    return launch_moe_route_scored(score, dtype, logits_dev, logits_stride, bias_dev, n_tokens, n_experts, n_groups, groups_kept, group_top, k, renormalise, weight_scale, idx_dev, weight_dev,
+                                   as_stream(stream));
+}
+
+// What cml_token_log_probs serves: 0, or the status that refuses it.
+static int bad_scoring(int64_t n_rows, int64_t vocab, int n_top) {
+    if (n_rows < 0 || n_rows > (1 << 24) || vocab < 1 || vocab > (1 << 30)) return fail(CML_ERR_SHAPE, "%lld rows of %lld logits", (long long)n_rows, (long long)vocab);
+    if (n_top < 0 || n_top > 64) return fail(CML_ERR_SHAPE, "the best %d tokens (0 to 64)", n_top);
+    return CML_OK;
+}
+
+size_t cml_token_log_probs_workspace_bytes(int64_t n_rows, int64_t vocab, int n_top) {
+    return bad_scoring(n_rows, vocab, n_top) || n_rows == 0 ? 0 : token_log_probs_workspace(n_rows, vocab, n_top);
+}
+
+int cml_token_log_probs(int dtype, const void *logits_dev, int64_t logits_stride, int64_t n_rows, int64_t vocab, const int32_t *target_dev, int n_top, float *log_prob_dev, int32_t *rank_dev,
+                        float *entropy_dev, int32_t *top_ids_dev, float *top_log_probs_dev, void *workspace_dev, size_t workspace_bytes, cml_stream_t stream) {
+    if (int rc = check_ready()) return rc;
+    if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
+    if (int rc = bad_scoring(n_rows, vocab, n_top)) return rc;
+    if (n_rows == 0) return CML_OK;
+    if (int rc = bad_rows("logits", logits_dev, logits_stride, vocab, n_rows, type_bytes(dtype))) return rc;
+    if (int rc = bad_f32("target", target_dev)) return rc;
+    if (int rc = bad_f32("log_prob", log_prob_dev)) return rc;
+    if (rank_dev)
+        if (int rc = bad_f32("rank", rank_dev)) return rc;
+    if (entropy_dev)
+        if (int rc = bad_f32("entropy", entropy_dev)) return rc;
+    if (n_top > 0) {
+        if (int rc = bad_f32("top_ids", top_ids_dev)) return rc;
+        if (int rc = bad_f32("top_log_probs", top_log_probs_dev)) return rc;
+    }
+    const size_t need = token_log_probs_workspace(n_rows, vocab, n_top);
+    if (need && !workspace_dev) return fail(CML_ERR_INVALID, "null workspace");
+    if (workspace_bytes < need) return fail(CML_ERR_SHAPE, "workspace of %zu bytes: %zu are needed", workspace_bytes, need);
+    if (need && misaligned16(workspace_dev)) return fail(CML_ERR_INVALID, "the workspace must be 16-byte aligned");
+    return launch_token_log_probs(dtype, logits_dev, logits_stride, n_rows, vocab, target_dev, n_top, log_prob_dev, rank_dev, entropy_dev, top_ids_dev, top_log_probs_dev, workspace_dev,
+                                  as_stream(stream));
+}
+
 // ---- matvec / matmul --------------------------------------------------------------------------------
 
 // The packed-dot kernels serve 8, 4, 2 or 1 tokens per pass over the weight: 3, 5, 6 and 7 tokens

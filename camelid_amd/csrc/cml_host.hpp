@@ -199,6 +199,25 @@ int q6k_mfma_min_tokens(int64_t rows, int64_t n_sb);         // batch size from 
 bool q4k_lane_order();                                       // CAMELID_HIP_Q4K_LANE_ORDER: the reference wire row dot's generic 8-lane order, bit for bit
 bool q6k_lane_order();                                       // CAMELID_HIP_Q6K_LANE_ORDER: the reference CPU lanes' 8-lane order, bit for bit
 
+// Value types of the int8 lane and of scoring, by GGUF type id.
+inline bool known_type(int dtype) { return dtype == CML_F32 || dtype == CML_F16 || dtype == CML_BF16; }
+inline int type_bytes(int dtype) { return dtype == CML_F32 ? 4 : 2; }
+// int8_rows.hip: rows of a type (CML_F32 / CML_F16 / CML_BF16) to int8 with one scale each, and back; strides in elements
+int launch_add_rms_norm_i8(int dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const float *weight, float eps, int64_t n_tokens, int64_t cols,
+                           void *sum, int64_t sum_stride, float *normed, int8_t *q, int64_t q_stride, float *scales, hipStream_t st);
+int launch_quantize_i8(int dtype, const void *x, int64_t x_stride, int64_t n_rows, int64_t cols, int8_t *q, int64_t q_stride, float *scales, hipStream_t st);
+int launch_dequantize_i8(const int8_t *q, int64_t q_stride, const float *scales, int64_t n_rows, int64_t cols, int dtype, void *out, int64_t out_stride, hipStream_t st);
+// matmul_i8.hip
+int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int64_t n_tokens, const int8_t *w, int64_t w_stride, const float *w_scales, int64_t rows, int64_t cols,
+                     const float *bias, int dtype, void *out, int64_t out_stride, hipStream_t st);
+// moe_route.hip
+int launch_moe_route_scored(int score, int dtype, const void *logits, int64_t stride, const float *bias, int64_t n_tokens, int n_experts, int n_groups, int groups_kept, int group_top, int k,
+                            int renormalise, float weight_scale, int32_t *idx, float *weight, hipStream_t st);
+// token_log_probs.hip
+size_t token_log_probs_workspace(int64_t n_rows, int64_t vocab, int n_top);
+int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_t n_rows, int64_t vocab, const int32_t *target, int n_top, float *log_prob, int32_t *rank, float *entropy,
+                           int32_t *top_ids, float *top_log_probs, void *workspace, hipStream_t st);
+
 // Integer tuning knob read once from the environment (0 when unset).
 int env_int(const char *name, int dflt);
 

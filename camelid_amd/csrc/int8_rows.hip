@@ -1,0 +1,217 @@
+// Rows to 8 bits with one scale each: the activation side of the int8 product (matmul_i8.hip).
+//
+//   h = rnd(x + residual)                 the residual stream, rounded to its own type: what the next layer reads is what is normalised
+//   y = h * inv * weight, inv = 1 / sqrt(mean(h^2) + eps)
+//   scale = max|y| / 127, q = round(y / scale), ties to even
+//
+// A row stays in registers between its one read and its writes.  The quotient y / scale is h * weight * (127 / max|h * weight|): inv cancels, so
+// the sum of squares and the maximum are reduced together, behind one barrier.  Sums and products are f32; the only roundings to
+// fewer bits are the stream's type and the 8 bits themselves.
+#include "typed_rows.hpp"
+
+#pragma clang fp contract(off)
+
+namespace cml {
+
+struct NormRows {
+    const void *x, *residual;
+    const float *weight;
+    void *sum;
+    float *normed;
+    int8_t *q;
+    float *scales;
+    int64_t x_stride, residual_stride, sum_stride, q_stride;  // elements
+    int64_t n_rows;
+    int cols;
+    float eps;
+};
+
+// A row by THREADS threads that hold CH times eight values each; workgroups of 256 threads at least, so rows of one wave go four to a workgroup.
+// NORM: the norm above; otherwise y = x.
+template <class T, bool NORM, int THREADS, int CH>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rows_to_i8_kernel(NormRows a) {
+    typedef typename T::Bits Bits;
+    constexpr int kWaves = THREADS / 64, kRows = THREADS < 256 ? 256 / THREADS : 1;
+    __shared__ float s_sum[kWaves];
+    __shared__ uint32_t s_max[kWaves];
+    const int tid = threadIdx.x & (THREADS - 1), wave = tid >> 6, lane = tid & 63;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + (kRows > 1 ? threadIdx.x / THREADS : 0);
+    if (kRows > 1 && row >= a.n_rows) return;  // (such rows meet no barrier)
+    const Bits *x = static_cast<const Bits *>(a.x) + row * a.x_stride;
+    const Bits *r = NORM && a.residual ? static_cast<const Bits *>(a.residual) + row * a.residual_stride : nullptr;
+    float h[CH][8], hw[CH][8];
+    float sum = 0.0f;
+    uint32_t top = 0;  // |h * weight| as bits: they order like the values, and a NaN is above all
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const int i = (c * THREADS + tid) * 8;
+        if (i + 8 <= a.cols) {
+            load8<T>(x + i, h[c]);
+            if (NORM && r) {
+                float add[8];
+                load8<T>(r + i, add);
+#pragma unroll
+                for (int j = 0; j < 8; j++) h[c][j] = rounded<T>(h[c][j] + add[j]);
+            }
+            if (NORM) load8<TypeF32>(a.weight + i, hw[c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                h[c][j] = hw[c][j] = 0.0f;
+                if (i + j < a.cols) {
+                    h[c][j] = load_value<T>(x + i + j);
+                    if (NORM && r) h[c][j] = rounded<T>(h[c][j] + load_value<T>(r + i + j));
+                    if (NORM) hw[c][j] = a.weight[i + j];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            hw[c][j] = NORM ? h[c][j] * hw[c][j] : h[c][j];
+            if (NORM) sum = fmaf(h[c][j], h[c][j], sum);
+            top = max(top, __builtin_bit_cast(uint32_t, hw[c][j]) & 0x7fffffffu);
+        }
+    }
+    if (NORM && a.sum) {
+        Bits *out = static_cast<Bits *>(a.sum) + row * a.sum_stride;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int i = (c * THREADS + tid) * 8;
+            if (i + 8 <= a.cols) {
+                store8<T>(out + i, h[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (i + j < a.cols) store_value<T>(out + i + j, h[c][j]);
+            }
+        }
+    }
+    if (NORM) sum = wave_allsum(sum);
+    top = static_cast<uint32_t>(wave_allmax_i32(static_cast<int>(top)));
+    if constexpr (kWaves > 1) {
+        if (lane == 0) {
+            s_sum[wave] = sum;
+            s_max[wave] = top;
+        }
+        __syncthreads();
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            sum = sum + s_sum[w];
+            top = max(top, s_max[w]);
+        }
+    }
+    float most = __builtin_bit_cast(float, top);
+    const float inv = NORM ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : 1.0f;
+    const float scale = most * inv / 127.0f;
+    // 127 / most of a row of tiny values would be infinite: such a row is lifted by 2^64 first
+    const float lift = most < 1e-30f ? 18446744073709551616.0f : 1.0f;
+    most = most * lift;
+    const bool live = most > 0.0f && fabsf(scale) < INFINITY;  // an empty row, or one with an infinity or a NaN in it (its scale is NaN or infinite): no quants
+    const float to_q = live ? 127.0f / most : 0.0f;
+    if (tid == 0) a.scales[row] = scale;
+    int8_t *q = a.q + row * a.q_stride;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        const int i = (c * THREADS + tid) * 8;
+        int v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = live ? static_cast<int>(fminf(fmaxf(rintf(hw[c][j] * lift * to_q), -127.0f), 127.0f)) : 0;
+        if (i + 8 <= a.cols) {
+            typedef uint32_t v2u __attribute__((ext_vector_type(2), aligned(1)));
+            *reinterpret_cast<v2u *>(q + i) = v2u{pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i + j < a.cols) q[i + j] = static_cast<int8_t>(v[j]);
+        }
+    }
+    if (NORM && a.normed) {
+        float *out = a.normed + row * a.cols;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int i = (c * THREADS + tid) * 8;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = hw[c][j] * inv;
+            if (i + 8 <= a.cols) {
+                store8<TypeF32>(out + i, y);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (i + j < a.cols) out[i + j] = y[j];
+            }
+        }
+    }
+}
+
+template <class T, bool NORM, int THREADS, int CH>
+static int launch_rows(const NormRows &a, hipStream_t st) {
+    constexpr int kThreads = THREADS < 256 ? 256 : THREADS, kRows = kThreads / THREADS;
+    hipLaunchKernelGGL((rows_to_i8_kernel<T, NORM, THREADS, CH>), dim3(static_cast<unsigned>((a.n_rows + kRows - 1) / kRows)), dim3(kThreads), 0, st, a);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+
+template <class T, bool NORM>
+static int launch_rows_typed(const NormRows &a, hipStream_t st) {
+    if (a.cols <= 512) return launch_rows<T, NORM, 64, 1>(a, st);
+    if (a.cols <= 2048) return launch_rows<T, NORM, 256, 1>(a, st);
+    if (a.cols <= 4096) return launch_rows<T, NORM, 256, 2>(a, st);
+    if (a.cols <= 8192) return launch_rows<T, NORM, 256, 4>(a, st);
+    if (a.cols <= 16384) return launch_rows<T, NORM, 1024, 2>(a, st);
+    if (a.cols <= 32768) return launch_rows<T, NORM, 1024, 4>(a, st);
+    return launch_rows<T, NORM, 1024, 8>(a, st);
+}
+
+int launch_add_rms_norm_i8(int dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const float *weight, float eps, int64_t n_tokens, int64_t cols,
+                           void *sum, int64_t sum_stride, float *normed, int8_t *q, int64_t q_stride, float *scales, hipStream_t st) {
+    const NormRows a{x, residual, weight, sum, normed, q, scales, x_stride, residual_stride, sum_stride, q_stride, n_tokens, static_cast<int>(cols), eps};
+    CML_COUNT_LAUNCH("i8.add_rms_norm");
+    return with_type(dtype, [&](auto t) { return launch_rows_typed<decltype(t), true>(a, st); });
+}
+
+int launch_quantize_i8(int dtype, const void *x, int64_t x_stride, int64_t n_rows, int64_t cols, int8_t *q, int64_t q_stride, float *scales, hipStream_t st) {
+    const NormRows a{x, nullptr, nullptr, nullptr, nullptr, q, scales, x_stride, 0, 0, q_stride, n_rows, static_cast<int>(cols), 0.0f};
+    CML_COUNT_LAUNCH("i8.quantize");
+    return with_type(dtype, [&](auto t) { return launch_rows_typed<decltype(t), false>(a, st); });
+}
+
+// out = q * scale, sixteen values a thread.
+template <class T>
+__global__ __launch_bounds__(256) void dequantize_i8_kernel(const int8_t *__restrict__ q, int64_t q_stride, const float *__restrict__ scales, int cols, int chunks,
+                                                            typename T::Bits *__restrict__ out, int64_t out_stride) {
+    const int64_t row = blockIdx.x / static_cast<unsigned>(chunks);
+    const int i = (static_cast<int>(blockIdx.x - row * chunks) * 256 + threadIdx.x) * 16;
+    if (i >= cols) return;
+    const int8_t *from = q + row * q_stride + i;
+    typename T::Bits *to = out + row * out_stride + i;
+    const float s = scales[row];
+    if (i + 16 <= cols) {
+        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(1)));
+        const v4u p = *reinterpret_cast<const v4u *>(from);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = static_cast<float>(static_cast<int8_t>(p[2 * k + j / 4] >> (8 * (j % 4)))) * s;
+            store8<T>(to + 8 * k, v);
+        }
+    } else {
+        for (int j = 0; i + j < cols; j++) store_value<T>(to + j, static_cast<float>(from[j]) * s);
+    }
+}
+
+int launch_dequantize_i8(const int8_t *q, int64_t q_stride, const float *scales, int64_t n_rows, int64_t cols, int dtype, void *out, int64_t out_stride, hipStream_t st) {
+    const int chunks = static_cast<int>((cols + 4095) / 4096);
+    CML_COUNT_LAUNCH("i8.dequantize");
+    return with_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL(dequantize_i8_kernel<T>, dim3(static_cast<unsigned>(n_rows * chunks)), dim3(256), 0, st, q, q_stride, scales, static_cast<int>(cols), chunks,
+                           static_cast<typename T::Bits *>(out), out_stride);
+        CML_HIP_TRY(hipGetLastError());
+        return CML_OK;
+    });
+}
+
+}  // namespace cml

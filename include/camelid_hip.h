@@ -418,6 +418,70 @@ int cml_moe_weighted_sum(const float *y_dev, const int32_t *route_to_assignment_
                          const float *weight_dev, int64_t n_tokens, int k, int64_t hidden,
                          float *out_dev, cml_stream_t stream);
 
+/* ==== the int8 lane and scoring ================================================================
+ * Rows of f32, f16 or bf16 values (`dtype`: the GGUF type ids below), strides in elements between the
+ * starts of rows (at least the row's length), any element-aligned address.  None of these has a
+ * counterpart in the reference, whose activations are f32 and whose 8-bit forms scale blocks. */
+#define CML_F32 0
+#define CML_F16 1
+#define CML_BF16 30
+
+/* Residual addition, RMS norm and 8-bit output of every token, in one pass:
+ *   h = x + residual, rounded to dtype     -> sum_dev (nullable; may be x or residual itself)
+ *   y = h * weight / sqrt(mean(h^2) + eps) -> normed_dev (f32[n_tokens*cols], nullable)
+ *   scale = max|y| / 127 -> scales_dev f32[n_tokens];  round(y / scale), ties to even -> q_dev
+ * residual_dev null: h = x.  weight_dev f32[cols].  Sums in f32.  A row of zeros has scale 0 and quants
+ * 0; a row whose values or squares leave the finite numbers has scale NaN or infinite and quants 0.  Rows of up to
+ * 65536 values. */
+int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const void *residual_dev,
+                        int64_t residual_stride, const float *weight_dev, float eps, int64_t n_tokens,
+                        int64_t cols, void *sum_dev, int64_t sum_stride, float *normed_dev,
+                        int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream);
+/* The quantizer alone, y = x: activations that no norm precedes, and weights (one scale per weight row). */
+int cml_quantize_i8(int dtype, const void *x_dev, int64_t x_stride, int64_t n_rows, int64_t cols,
+                    int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream);
+/* q * scale, rounded to dtype. */
+int cml_dequantize_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev, int64_t n_rows,
+                      int64_t cols, int dtype, void *out_dev, int64_t out_stride, cml_stream_t stream);
+/* out[t][r] = (sum over c of q[t][c] * w[r][c]) * scales[t] * w_scales[r] + bias[r], the sum an exact
+ * 32-bit integer, the rest in f32, rounded once to dtype.  q int8[n_tokens][cols], w int8[rows][cols]
+ * (any of the 256 values), bias_dev f32[rows] or null.  cols up to 131071.  The bits depend neither on the
+ * number of tokens nor on the kernel that serves the call.  Rows that start on 16-byte boundaries (base and stride, of q and
+ * w both) run on the faster kernels. */
+int cml_matmul_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev, int64_t n_tokens,
+                  const int8_t *w_dev, int64_t w_stride, const float *w_scales_dev, int64_t rows,
+                  int64_t cols, const float *bias_dev, int dtype, void *out_dev, int64_t out_stride,
+                  cml_stream_t stream);
+/* Routing with the forms that cml_moe_route_top_k and cml_moe_route_softmax_top_k do not have; its outputs
+ * are theirs (idx int32[n_tokens*k], weight f32[n_tokens*k]) and go to cml_moe_plan / cml_moe_ffn.
+ *   score = softmax over all experts, or the sigmoid of each logit
+ *   key = score + bias (bias_dev f32[n_experts] or null: then the logit, which orders the same)
+ *   n_groups > 1: consecutive experts form groups of n_experts / n_groups; a group's worth is the sum of its
+ *     group_top (1 or 2) best keys (without a bias and for 2: of those experts' scores), the groups_kept best groups stay
+ *   the k best keys of the groups that stay, in descending order, ties to the lower index throughout
+ *   weight = score, divided by the sum of the chosen scores if renormalise, times weight_scale
+ * An expert whose logit or key is -inf or NaN takes no part; slots without an expert have id -1 and weight 0.
+ * +inf counts as the largest finite logit.  Up to 1024 experts, 64 groups, k up to 64. */
+enum { CML_ROUTE_SOFTMAX = 0, CML_ROUTE_SIGMOID = 1 };
+int cml_moe_route_scored(int score, int dtype, const void *logits_dev, int64_t logits_stride,
+                         const float *bias_dev, int64_t n_tokens, int n_experts, int n_groups,
+                         int groups_kept, int group_top, int k, int renormalise, float weight_scale,
+                         int32_t *idx_dev, float *weight_dev, cml_stream_t stream);
+/* For every row of logits and its given token target[row]: the token's log probability; its rank (1 = the
+ * largest logit; ties count lower indices first; nullable); the row's entropy in nats (nullable); the
+ * n_top (0 to 64) best tokens in order, ties to the lower index, with their log probabilities
+ * (top_ids int32[n_rows*n_top], top_log_probs f32; null for n_top = 0).  Sums in f32.
+ * -inf is a masked token: probability 0, never an alternative; slots without a token have id -1 and
+ * -inf.  A row of masked tokens: log probability -inf, entropy 0.  A target outside the
+ * vocabulary: log probability NaN, rank 0.  NaN or +inf in a row: NaN in log probabilities and entropy.
+ * workspace_dev needs cml_token_log_probs_workspace_bytes(...) bytes (0 for many rows; 16-byte aligned); a vocabulary of up to 2^30. */
+size_t cml_token_log_probs_workspace_bytes(int64_t n_rows, int64_t vocab, int n_top);
+int cml_token_log_probs(int dtype, const void *logits_dev, int64_t logits_stride, int64_t n_rows,
+                        int64_t vocab, const int32_t *target_dev, int n_top, float *log_prob_dev,
+                        int32_t *rank_dev, float *entropy_dev, int32_t *top_ids_dev,
+                        float *top_log_probs_dev, void *workspace_dev, size_t workspace_bytes,
+                        cml_stream_t stream);
+
 /* ---- weight quantizer tool (reference quantize_block_q8_0 / q4_0 / q4_k,
  *      src/quantize.rs:98-244): f32 values -> GGUF wire bytes on the host, in
  *      whole blocks, on `threads` threads.  Q6_K has no counterpart in the

@@ -22,6 +22,13 @@ pub const CML_Q8_0: i32 = 8;
 pub const CML_Q4_K: i32 = 12;
 pub const CML_Q6_K: i32 = 14;
 
+// Value types of the int8 lane and of scoring, and the scores of cml_moe_route_scored.
+pub const CML_F32: i32 = 0;
+pub const CML_F16: i32 = 1;
+pub const CML_BF16: i32 = 30;
+pub const CML_ROUTE_SOFTMAX: i32 = 0;
+pub const CML_ROUTE_SIGMOID: i32 = 1;
+
 pub const CML_OK: i32 = 0;
 pub const CML_ERR_UNAVAILABLE: i32 = 1;
 pub const CML_ERR_INVALID: i32 = 2;
@@ -135,6 +142,15 @@ extern "C" {
                                max_assignments_per_expert: i64, out_dev: *mut f32, stream: Stream) -> i32;
     pub fn cml_moe_weighted_sum(y_dev: *const f32, route_to_assignment_dev: *const i32, weight_dev: *const f32, n_tokens: i64, k: i32,
                                 hidden: i64, out_dev: *mut f32, stream: Stream) -> i32;
+    // ---- the int8 lane and scoring (no counterpart in the reference); dtype: CML_F32 / CML_F16 / CML_BF16
+    pub fn cml_add_rms_norm_i8(dtype: i32, x_dev: *const c_void, x_stride: i64, residual_dev: *const c_void, residual_stride: i64, weight_dev: *const f32, eps: f32, n_tokens: i64, cols: i64, sum_dev: *mut c_void, sum_stride: i64, normed_dev: *mut f32, q_dev: *mut i8, q_stride: i64, scales_dev: *mut f32, stream: Stream) -> i32;
+    pub fn cml_quantize_i8(dtype: i32, x_dev: *const c_void, x_stride: i64, n_rows: i64, cols: i64, q_dev: *mut i8, q_stride: i64, scales_dev: *mut f32, stream: Stream) -> i32;
+    pub fn cml_dequantize_i8(q_dev: *const i8, q_stride: i64, scales_dev: *const f32, n_rows: i64, cols: i64, dtype: i32, out_dev: *mut c_void, out_stride: i64, stream: Stream) -> i32;
+    pub fn cml_matmul_i8(q_dev: *const i8, q_stride: i64, scales_dev: *const f32, n_tokens: i64, w_dev: *const i8, w_stride: i64, w_scales_dev: *const f32, rows: i64, cols: i64, bias_dev: *const f32, dtype: i32, out_dev: *mut c_void, out_stride: i64, stream: Stream) -> i32;
+    pub fn cml_moe_route_scored(score: i32, dtype: i32, logits_dev: *const c_void, logits_stride: i64, bias_dev: *const f32, n_tokens: i64, n_experts: i32, n_groups: i32, groups_kept: i32, group_top: i32, k: i32, renormalise: i32, weight_scale: f32, idx_dev: *mut i32, weight_dev: *mut f32, stream: Stream) -> i32;
+    pub fn cml_token_log_probs_workspace_bytes(n_rows: i64, vocab: i64, n_top: i32) -> usize;
+    pub fn cml_token_log_probs(dtype: i32, logits_dev: *const c_void, logits_stride: i64, n_rows: i64, vocab: i64, target_dev: *const i32, n_top: i32, log_prob_dev: *mut f32, rank_dev: *mut i32, entropy_dev: *mut f32, top_ids_dev: *mut i32, top_log_probs_dev: *mut f32, workspace_dev: *mut c_void, workspace_bytes: usize, stream: Stream) -> i32;
+
     // ---- host-side helpers and the host-pointer seams
     pub fn cml_quantize_weights_host(fmt: i32, src: *const f32, n_values: usize, dst: *mut u8, threads: i32) -> i32;
     pub fn cml_try_linear_rows(fmt: i32, input_scales: *const f32, input_quants: *const i8, weight_wire: *const u8, weight_nbytes: usize,

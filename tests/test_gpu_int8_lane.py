@@ -1,0 +1,234 @@
+"""The int8 lane through the C ABI against plain numpy: residual + RMS norm + quantizer, the quantizer alone, its inverse, and the product.
+
+Tolerances.  A row's sum of squares is a chain of at most 64 fused multiply-adds and 26 additions: 90 roundings of 2^-24, half of
+that (2.7e-6) on the inverse root, and five more roundings behind it: 4e-6 on scale and normalised values.  A quant is the rounding of a quotient
+that four roundings have moved by at most 127 * 4 * 2^-24 = 3.1e-5.  The residual stream, the dequantized values and the product are
+defined operation by operation: their bits are compared.
+"""
+import numpy as np
+import pytest
+
+from camelid_amd import binding as B
+from camelid_amd.binding import check, lib
+from tests import gpu_util as G
+from tests.typed_rows import BITS, TYPES, Rows, from_bits, to_bits
+
+pytestmark = pytest.mark.gpu
+REL = 4e-6
+
+
+def f32(a):
+    return Rows(np.ascontiguousarray(a, np.float32).reshape(1, -1))
+
+
+def norm(t, x, residual, weight, eps, *, pad=0, offset=0, in_place=False, want_sum=True, want_normed=True, stream=None):
+    """(sum bits, normed, q, scales) of one call on bit patterns x, residual."""
+    B.init(0)
+    n, cols = x.shape
+    X = Rows(x, cols + pad, offset)
+    R = Rows(residual, cols + pad, offset) if residual is not None else None
+    S = (R if R else X) if in_place else Rows.empty(n, cols, BITS[t], cols + pad, offset) if want_sum else None
+    N = Rows.empty(n, cols, np.float32) if want_normed else None
+    Q, D, W = Rows.empty(n, cols, np.int8, cols + pad, offset), Rows.empty(1, n, np.float32), f32(weight)
+    G.say(f"add_rms_norm_i8 {t} {n}x{cols} pad={pad} offset={offset} residual={R is not None}")
+    check(lib().cml_add_rms_norm_i8(TYPES[t], X.ptr, X.stride, R.ptr if R else None, R.stride if R else 0, W.ptr, eps, n, cols, S.ptr if S else None, S.stride if S else 0,
+                                    N.ptr if N else None, Q.ptr, Q.stride, D.ptr, stream))
+    check(lib().cml_stream_sync(stream))
+    return S.get() if S else None, N.get() if N else None, Q.get(), D.get()[0]
+
+
+def check_norm(t, x, residual, weight, eps, got):
+    sum_bits, normed, q, scales = got
+    h = from_bits(x, t)
+    if residual is not None:
+        h = from_bits(to_bits(h + from_bits(residual, t), t), t)
+    if sum_bits is not None:
+        assert np.array_equal(sum_bits, to_bits(h, t))
+    h = h.astype(np.float64)
+    y = h / np.sqrt(np.mean(h * h, axis=1, keepdims=True) + eps) * weight.astype(np.float64)
+    step = np.abs(y).max(axis=1) / 127
+    if normed is not None:
+        assert np.all(np.abs(normed - y) <= REL * np.abs(y))
+    assert np.all(np.abs(scales - step) <= REL * step)
+    live = step > 0
+    assert np.all(q[~live] == 0)
+    assert np.all(np.abs(q[live] - y[live] / step[live, None]) <= 0.5 + 3.1e-5)
+    assert np.all(np.abs(q[live].astype(int)).max(axis=1) == 127)
+
+
+# one value; odd; the last of one wave; either side of every number of values a thread holds; the longest
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,cols,pad,offset", [(1, 1, 0, 0), (5, 7, 3, 1), (9, 512, 0, 0), (3, 513, 0, 0), (4, 2048, 8, 8), (2, 2049, 1, 3), (3, 4096, 0, 0), (2, 4100, 0, 0),
+                                               (2, 8193, 0, 1), (1, 16384, 0, 0), (1, 16391, 0, 0), (1, 40000, 0, 0), (1, 65536, 0, 0), (2100, 96, 0, 0)])
+def test_norm_sizes(t, n, cols, pad, offset):
+    rng = np.random.default_rng(cols + n)
+    channel = np.exp(0.5 * rng.standard_normal(cols))
+    x, r = to_bits(rng.standard_normal((n, cols)) * channel, t), to_bits(2 * rng.standard_normal((n, cols)) * channel, t)
+    w = (0.5 + rng.random(cols)).astype(np.float32)
+    check_norm(t, x, r, w, 1e-5, norm(t, x, r, w, 1e-5, pad=pad, offset=offset))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_norm_without_residual_in_place_and_without_the_optional_outputs(t):
+    rng = np.random.default_rng(3)
+    x, r = to_bits(rng.standard_normal((6, 1000)), t), to_bits(rng.standard_normal((6, 1000)), t)
+    w = (0.5 + rng.random(1000)).astype(np.float32)
+    w[5] = -2.0
+    full = norm(t, x, r, w, 1e-6)
+    check_norm(t, x, None, w, 1e-6, norm(t, x, None, w, 1e-6))
+    for got in (norm(t, x, r, w, 1e-6, in_place=True), norm(t, x, r, w, 1e-6, want_sum=False, want_normed=False)):
+        for a, b in zip(got, full):
+            assert a is None or np.array_equal(a, b)
+
+
+def test_norm_rows_of_zeros_tiny_values_infinities_and_nan():
+    cols = 600
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((7, cols)).astype(np.float32)
+    x[1] = 0.0
+    x[2] *= 1e-38       # (squares vanish; eps alone is left)
+    x[3, 17] = np.inf
+    x[4, 599] = np.nan
+    x[5] = 0.0
+    x[5, 0] = 1e-41     # subnormal
+    w = np.ones(cols, np.float32)
+    s, y, q, d = norm("f32", x.view(np.uint32), None, w, 1e-5)
+    keep = [0, 1, 2, 6]
+    check_norm("f32", x[keep].view(np.uint32), None, w, 1e-5, (s[keep], None, q[keep], d[keep]))
+    assert np.all(q[1] == 0) and d[1] == 0
+    assert not np.isfinite(d[3]) and not np.isfinite(d[4]) and np.all(q[3:5] == 0)
+    assert q[5, 0] == 127 and np.all(q[5, 1:] == 0)
+    w[9] = np.nan
+    s, y, q, d = norm("f32", x.view(np.uint32), None, w, 1e-5)
+    assert np.isnan(d[0]) and np.all(q[0] == 0)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,cols,pad", [(1, 1, 0), (6, 33, 2), (300, 512, 0), (3, 5000, 0), (2, 20001, 5)])
+def test_quantizer_alone_and_back(t, n, cols, pad):
+    B.init(0)
+    rng = np.random.default_rng(n)
+    x = to_bits(rng.standard_normal((n, cols)) * 3, t)
+    X, Q, D = Rows(x, cols + pad), Rows.empty(n, cols, np.int8, cols + pad), Rows.empty(1, n, np.float32)
+    O = Rows.empty(n, cols, BITS[t], cols + pad)
+    G.say(f"quantize_i8 / dequantize_i8 {t} {n}x{cols}")
+    check(lib().cml_quantize_i8(TYPES[t], X.ptr, X.stride, n, cols, Q.ptr, Q.stride, D.ptr, None))
+    check(lib().cml_dequantize_i8(Q.ptr, Q.stride, D.ptr, n, cols, TYPES[t], O.ptr, O.stride, None))
+    check(lib().cml_stream_sync(None))
+    v, q, d = from_bits(x, t).astype(np.float64), Q.get(), D.get()[0]
+    step = np.abs(v).max(axis=1) / 127
+    assert np.all(np.abs(d - step) <= 2.0 ** -23 * step)
+    assert np.all(np.abs(q - v / step[:, None]) <= 0.5 + 3.1e-5)
+    assert np.array_equal(O.get(), to_bits(q.astype(np.float32) * d[:, None], t))
+
+
+def product(t, q, w, s, ws, bias, *, q_pad=0, w_pad=0, out_pad=0, offset=0):
+    B.init(0)
+    n, rows, cols = q.shape[0], w.shape[0], q.shape[1]
+    Q, W, O = Rows(q, cols + q_pad, offset), Rows(w, cols + w_pad, offset), Rows.empty(n, rows, BITS[t], rows + out_pad)
+    S, WS, BI = f32(s), f32(ws), f32(bias) if bias is not None else None
+    G.say(f"matmul_i8 {t} tokens={n} rows={rows} cols={cols} pads={q_pad},{w_pad},{out_pad} offset={offset}")
+    check(lib().cml_matmul_i8(Q.ptr, Q.stride, S.ptr, n, W.ptr, W.stride, WS.ptr, rows, cols, BI.ptr if BI else None, TYPES[t], O.ptr, O.stride, None))
+    check(lib().cml_stream_sync(None))
+    return O.get()
+
+
+def want_product(t, q, w, s, ws, bias):
+    total = (q.astype(np.float64) @ w.astype(np.float64).T).astype(np.int64)  # exact: below 2^53
+    out = total.astype(np.float32) * s[:, None] * ws[None, :]
+    return to_bits(out if bias is None else out + bias[None, :], t)
+
+
+def operands(seed, n, rows, cols):
+    rng = np.random.default_rng(seed)
+    q, w = rng.integers(-128, 128, (n, cols)).astype(np.int8), rng.integers(-128, 128, (rows, cols)).astype(np.int8)
+    return q, w, (0.01 + rng.random(n)).astype(np.float32), (rng.random(rows) * 1e-3).astype(np.float32), rng.standard_normal(rows).astype(np.float32)
+
+
+# tokens: one, odd, either side of 16 / 32 / 64 / 128 / 256; rows and columns inside, at and past whole tiles
+@pytest.mark.parametrize("n,rows,cols", [(1, 1, 1), (1, 64, 16), (1, 4096, 4096), (2, 130, 48), (3, 1000, 2816), (8, 257, 528), (16, 4096, 512), (17, 96, 80), (33, 704, 2816), (37, 1003, 2048),
+                                         (64, 512, 4096), (65, 63, 1040), (100, 333, 14336), (128, 256, 256), (129, 257, 272), (200, 1000, 1024), (256, 512, 128), (300, 2050, 4096), (513, 769, 384),
+                                         (1024, 1024, 144), (1100, 1300, 2048)])
+def test_product_sizes(n, rows, cols):
+    q, w, s, ws, bias = operands(n + rows + cols, n, rows, cols)
+    t = ["f32", "f16", "bf16"][(n + rows) % 3]
+    assert np.array_equal(product(t, q, w, s, ws, bias), want_product(t, q, w, s, ws, bias))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,rows,cols,q_pad,w_pad,out_pad,offset", [(5, 70, 1, 0, 0, 0, 0), (5, 70, 77, 0, 0, 1, 0), (40, 100, 129, 0, 15, 0, 0), (70, 90, 256, 16, 32, 3, 0), (70, 90, 256, 1, 0, 0, 0),
+                                                                    (70, 90, 256, 0, 0, 0, 4), (3, 200, 100, 12, 12, 0, 16), (300, 300, 500, 12, 12, 5, 0), (260, 520, 1000, 8, 8, 0, 0)])
+def test_product_strides_alignments_and_no_bias(t, n, rows, cols, q_pad, w_pad, out_pad, offset):
+    q, w, s, ws, _ = operands(cols, n, rows, cols)
+    assert np.array_equal(product(t, q, w, s, ws, None, q_pad=q_pad, w_pad=w_pad, out_pad=out_pad, offset=offset), want_product(t, q, w, s, ws, None))
+
+
+@pytest.mark.parametrize("n", [1, 20, 300])
+def test_product_extremes_stay_exact(n):
+    cols, rows = 131071 // 16 * 16, 33
+    q, w = np.full((n, cols), -128, np.int8), np.full((rows, cols), -128, np.int8)
+    w[1::2] = 127
+    q[::3, ::2] = 127
+    one, rows_one = np.ones(n, np.float32), np.ones(rows, np.float32)
+    assert np.array_equal(product("f32", q, w, one, rows_one, None), want_product("f32", q, w, one, rows_one, None))
+
+
+def test_product_of_a_token_does_not_depend_on_the_batch():
+    q, w, s, ws, bias = operands(11, 700, 600, 2048)
+    full = product("f32", q, w, s, ws, bias)
+    for n in (1, 2, 16, 17, 40, 64, 130, 257):
+        assert np.array_equal(product("f32", q[:n], w, s[:n], ws, bias), full[:n])
+
+
+def test_scales_that_are_not_finite_reach_their_cells_alone():
+    q, w, s, ws, _ = operands(12, 20, 50, 64)
+    s[3], ws[7] = np.nan, np.inf
+    got = from_bits(product("f32", q, w, s, ws, None), "f32")
+    assert np.all(np.isnan(got[3])) and not np.any(np.isfinite(got[:, 7]))
+    rest = np.delete(np.delete(got, 3, 0), 7, 1)
+    assert np.all(np.isfinite(rest))
+
+
+def test_refusals():
+    B.init(0)
+    L = lib()
+    x, q, d, o = Rows.empty(4, 64, np.float32), Rows.empty(4, 64, np.int8), Rows.empty(1, 4, np.float32), Rows.empty(4, 64, np.float32)
+    wt = f32(np.ones(64))
+    ok_norm = dict(dtype=0, x=x.ptr, xs=64, r=None, rs=0, w=wt.ptr, eps=1e-5, n=4, cols=64, s=None, ss=0, y=None, q=q.ptr, qs=64, d=d.ptr)
+
+    def norm_status(**kw):
+        a = {**ok_norm, **kw}
+        return L.cml_add_rms_norm_i8(a["dtype"], a["x"], a["xs"], a["r"], a["rs"], a["w"], a["eps"], a["n"], a["cols"], a["s"], a["ss"], a["y"], a["q"], a["qs"], a["d"], None)
+
+    assert norm_status() == 0 and norm_status(n=0) == 0 and norm_status(cols=0) == 0 and norm_status(n=1, xs=0, qs=0) == 0
+    for kw in (dict(dtype=2), dict(x=None), dict(w=None), dict(q=None), dict(d=None), dict(x=x.ptr + 2), dict(w=wt.ptr + 1), dict(y=x.ptr + 2), dict(r=x.ptr + 1, rs=64)):
+        assert norm_status(**kw) == 2, kw
+        assert L.cml_last_error()
+    for kw in (dict(n=-1), dict(cols=-1), dict(xs=63), dict(qs=63), dict(r=x.ptr, rs=8), dict(s=o.ptr, ss=63), dict(n=(1 << 30) + 1)):
+        assert norm_status(**kw) == 3, kw
+    assert norm_status(cols=65537, xs=65537, qs=65537, n=1) == 6
+
+    assert L.cml_quantize_i8(0, x.ptr, 64, 4, 64, q.ptr, 64, d.ptr, None) == 0
+    assert L.cml_quantize_i8(7, x.ptr, 64, 4, 64, q.ptr, 64, d.ptr, None) == 2
+    assert L.cml_quantize_i8(0, x.ptr, 63, 4, 64, q.ptr, 64, d.ptr, None) == 3
+    assert L.cml_quantize_i8(0, x.ptr, 1 << 20, 1, 1 << 20, q.ptr, 1 << 20, d.ptr, None) == 6
+    assert L.cml_dequantize_i8(q.ptr, 64, d.ptr, 4, 64, 0, o.ptr, 64, None) == 0
+    assert L.cml_dequantize_i8(q.ptr, 64, None, 4, 64, 0, o.ptr, 64, None) == 2
+    assert L.cml_dequantize_i8(q.ptr, 64, d.ptr, 4, 64, 3, o.ptr, 64, None) == 2
+    assert L.cml_dequantize_i8(q.ptr, 64, d.ptr, 4, 64, 0, o.ptr, 60, None) == 3
+    assert L.cml_dequantize_i8(q.ptr, 64, d.ptr, -4, 64, 0, o.ptr, 64, None) == 3
+
+    w, ws = Rows.empty(8, 64, np.int8), f32(np.ones(8))
+    ok = dict(q=q.ptr, qs=64, s=d.ptr, n=4, w=w.ptr, wst=64, ws=ws.ptr, rows=8, cols=64, b=None, dtype=0, o=o.ptr, os=64)
+
+    def status(**kw):
+        a = {**ok, **kw}
+        return L.cml_matmul_i8(a["q"], a["qs"], a["s"], a["n"], a["w"], a["wst"], a["ws"], a["rows"], a["cols"], a["b"], a["dtype"], a["o"], a["os"], None)
+
+    assert status() == 0 and status(n=0) == 0 and status(rows=0) == 0
+    for kw in (dict(q=None), dict(s=None), dict(w=None), dict(ws=None), dict(o=None), dict(dtype=24), dict(o=o.ptr + 2), dict(s=d.ptr + 1), dict(b=d.ptr + 2)):
+        assert status(**kw) == 2, kw
+    for kw in (dict(n=-1), dict(rows=-1), dict(cols=0), dict(cols=131072, qs=131072, wst=131072), dict(qs=63), dict(wst=1), dict(os=7)):
+        assert status(**kw) == 3, kw
+    assert status(n=(1 << 20) + 1) == 6
+    check(L.cml_stream_sync(None))
