@@ -784,7 +784,7 @@ int cml_matmul_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev
     if (int rc = check_ready()) return rc;
     if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
     if (n_tokens < 0 || rows < 0 || cols <= 0 || cols > kMostI8Cols) return fail(CML_ERR_SHAPE, "%lld tokens, %lld rows of %lld values (1 to %lld)", (long long)n_tokens, (long long)rows, (long long)cols, (long long)kMostI8Cols);
-    if (n_tokens > (1 << 20) || rows > (1 << 27)) return fail(CML_ERR_UNSUPPORTED, "%lld tokens and %lld rows in one call", (long long)n_tokens, (long long)rows);
+    if (n_tokens > (1 << 20) || rows > (1 << 27) || n_tokens * rows > (1ll << 37)) return fail(CML_ERR_UNSUPPORTED, "%lld tokens and %lld rows in one call", (long long)n_tokens, (long long)rows);
     if (n_tokens == 0 || rows == 0) return CML_OK;
     if (int rc = bad_rows("q", q_dev, q_stride, cols, n_tokens, 1)) return rc;
     if (int rc = bad_rows("w", w_dev, w_stride, cols, rows, 1)) return rc;

@@ -2,6 +2,11 @@
 //   out[t][r] = rnd((sum_c q[t][c] * w[r][c]) * scales[t] * w_scales[r] + bias[r])
 // The sum is an exact 32-bit integer (rows of up to 131071 values: 2^14 * 131071 < 2^31), so no split of the contraction changes a bit.  It is
 // widened to f32 (24 bits), scaled in f32 and rounded once to the output's type.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "gemm_wide.hpp"
 #include "typed_rows.hpp"
 
 #pragma clang fp contract(off)
@@ -77,9 +82,590 @@ __global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulI8 a) {
         for (int j = 0; j < 2; j++) store_cells<T>(a, t0 + wt + 16 * j + n, r0 + wr + 16 * i + 4 * (lane >> 4), acc[i][j]);
 }
 
+// ---- few tokens -----------------------------------------------------------------------------------------
+// Up to 16 tokens: the weight's bytes are the time.  A workgroup owns 16 weight rows; its waves take the 128-byte lines of the rows in turn, so that all
+// of a short row is requested at once, and their sums meet in LDS.  Operands go from memory to registers: lane 16 k + n holds 16 bytes of row
+// (token) n, and which bytes of the line does not matter as long as both operands agree.  Any alignment, any length.
+template <class T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void matmul_i8_few_kernel(MatmulI8 a) {
+    constexpr int U = 2;  // lines of every row in one batch of requests
+    __shared__ v4i_i8 part[WAVES - 1][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, kq = lane >> 4;
+    const int r0 = blockIdx.x * 16;
+    typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+    const int8_t *w = a.w + min(r0 + n, a.rows - 1) * a.w_stride + 32 * kq, *q = a.q + min(n, a.n_tokens - 1) * a.q_stride + 32 * kq;
+    v4i_i8 acc = {};
+    const int lines = a.cols >> 7;
+    struct Line {
+        v4i_i8 w[2], q[2];
+    };
+    auto load = [&](int line, Line &l) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l.w[h] = __builtin_nontemporal_load(reinterpret_cast<const v4i_any *>(w + line * 128 + 16 * h));
+            l.q[h] = *reinterpret_cast<const v4i_any *>(q + line * 128 + 16 * h);
+        }
+    };
+    auto multiply = [&](const Line &l) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(l.w[h], l.q[h], acc, 0, 0, 0);
+    };
+    int line = wave;
+    Line now[U], next[U];
+    constexpr int kBatch = U * WAVES, kLast = (U - 1) * WAVES;
+    if (line + kLast < lines) {  // whole batches, the next one requested while this one is multiplied
+#pragma unroll
+        for (int u = 0; u < U; u++) load(line + u * WAVES, now[u]);
+        for (; line + kBatch + kLast < lines; line += kBatch) {
+#pragma unroll
+            for (int u = 0; u < U; u++) load(line + kBatch + u * WAVES, next[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) multiply(now[u]);
+#pragma unroll
+            for (int u = 0; u < U; u++) now[u] = next[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) multiply(now[u]);
+        line += kBatch;
+    }
+    for (; line < lines; line += WAVES) {
+        load(line, now[0]);
+        multiply(now[0]);
+    }
+    if ((a.cols & 127) && lines % WAVES == wave) {  // the rest of the rows, zeros behind their ends
+        auto piece = [&](const int8_t *p, int c) {
+            if (c + 16 <= a.cols) return static_cast<v4i_i8>(*reinterpret_cast<const v4i_any *>(p));
+            v4i_i8 v = {};
+            for (int j = 0; c + j < a.cols; j++) v[j >> 2] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * (j & 3)));
+            return v;
+        };
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int c = lines * 128 + 32 * kq + 16 * h;
+            now[0].w[h] = piece(w + lines * 128 + 16 * h, c);
+            now[0].q[h] = piece(q + lines * 128 + 16 * h, c);
+        }
+        multiply(now[0]);
+    }
+    if (wave > 0) part[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int k = 0; k < WAVES - 1; k++) acc += part[k][lane];
+    store_cells<T>(a, n, r0 + 4 * kq, acc);
+}
+
+template <class T, int WAVES>
+static int launch_few(const MatmulI8 &a, hipStream_t st) {
+    hipLaunchKernelGGL((matmul_i8_few_kernel<T, WAVES>), dim3(static_cast<unsigned>((a.rows + 15) / 16)), dim3(64 * WAVES), 0, st, a);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+
+// ---- tiles --------------------------------------------------------------------------------------------
+// Rows on 16-byte boundaries.  WR x WT waves of MT x NT tiles of 32 x 32 cells; a step is 128 values of the contraction: whole lines of both operands
+// go to LDS without passing through registers, into the oldest of STAGES steps as soon as it has been read.  Slot p of an LDS row (16 bytes) holds piece p ^ key(row), so that the eight rows that
+// eight neighbouring lanes read lie in different banks.
+//
+// The instruction's 32 rows are the tile's in another order: a lane ends up with 16 neighbouring weight rows of its token and stores them whole.
+typedef int v16i_i8 __attribute__((ext_vector_type(16)));
+
+struct TileGrid {
+    int n_row_blocks, n_token_blocks, group;
+};
+
+// The at-th tile in the order of bands of `group` token blocks, row block after row block: neighbours share rows of both operands.  Consecutive workgroup
+// ids go to the eight XCDs in turn; each XCD gets a run of its own of that order, so that what its tiles share comes through its L2 once.
+__device__ __forceinline__ void tile_of(const TileGrid &g, int at, int &row_block, int &token_block, int &wide) {
+    const int band = at / (g.group * g.n_row_blocks), in = at - band * g.group * g.n_row_blocks;
+    wide = min(g.group, g.n_token_blocks - band * g.group);
+    row_block = in / wide;
+    token_block = band * g.group + in - row_block * wide;
+}
+
+// A pointer that is the same in all lanes, for an operand that has to be in scalar registers.
+__device__ __forceinline__ const int8_t *wave_uniform(const int8_t *p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)), high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const int8_t *>(static_cast<uint64_t>(high) << 32 | low);
+}
+
+// One tile's work by a workgroup of WR x WT waves.  SPLIT: the tile has 1 / SPLIT of the rows.  FULL: every row and token of the tile is there.
+template <class T, int WR, int WT, int MT, int NT, int STAGES, bool ONCE, bool FULL>
+struct TileWork {
+    static constexpr int KB = 128;  // values of the contraction a step: a whole line of a row
+    static constexpr int kWaves = WR * WT, kThreads = 64 * kWaves, kRows = WR * MT * 32, kTokens = WT * NT * 32;
+    static constexpr int kPass = kThreads / 8;  // rows that one pass of the workgroup fetches
+    static constexpr int kStage = (kRows + kTokens) * KB, kFetches = (kRows + kTokens) / kPass, kWeightFetches = kRows / kPass;
+    static constexpr int kTouch = STAGES == 2, kParts = KB / 32;
+    static constexpr int kScales = STAGES * kStage + kTouch * kWaves * 256, kLds = kScales + 8 * kRows;  // stages, what touch() fills, scales and bias of the rows
+    static_assert((kRows + kTokens) % kPass == 0 && kRows % kPass == 0, "whole passes of the workgroup");
+
+    const MatmulI8 &a;
+    const int8_t *lds;
+    uint32_t lds0;
+    int tid, lane, wave, wr, wt, m, half, row_a, n_steps;
+    int r0, t0;                 // of the tile that is fetched
+    uint32_t src[FULL ? 2 : kFetches];
+    const int8_t *touched;
+    bool touches;
+    uint32_t at_a, at_b;
+    v16i_i8 acc[MT][NT];
+    v4i_i8 fa[2][MT], fb[2][NT];
+
+    // (sixteen lanes read at a time; 64 banks are two rows of 128 bytes)
+    static __device__ __forceinline__ int key_w(int row) { return (row >> 1 & 3) | (row >> 2 & 4); }
+    static __device__ __forceinline__ int key_q(int row) { return row >> 1 & 7; }
+
+    __device__ __forceinline__ TileWork(const MatmulI8 &args, uint4 *smem) : a(args) {
+        lds = reinterpret_cast<const int8_t *>(smem);
+        lds0 = lds_address(smem);
+        tid = threadIdx.x;
+        lane = tid & 63;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        wr = wave / WT;
+        wt = wave - wr * WT;
+        m = lane & 31;
+        half = lane >> 5;
+        row_a = (m & 3) | (m >> 1 & 12) | (m << 2 & 16);  // instruction row 8a + 4b + c is the tile's 16b + 4a + c
+        n_steps = a.cols / KB;
+        at_a = (wr * MT * 32 + row_a) * KB + ((half ^ key_w(row_a)) << 4);  // of part 0; part s has piece 2 s + half: the address exclusive-or 32 s
+        at_b = (kRows + wt * NT * 32 + m) * KB + ((half ^ key_q(m)) << 4);
+    }
+
+    // Pass k of the workgroup takes LDS rows k * kPass ..; the weight's rows first, then the tokens'.  Rows past the end repeat the last one.
+    template <int SPLIT>
+    __device__ __forceinline__ void aim(int row, int token, int row_share, int wide, int token_share) {
+        constexpr int kMine = kRows / SPLIT;
+        r0 = row;
+        t0 = token;
+        int tid = this->tid;
+        asm volatile("" : "+v"(tid));  // (as in store)
+        const int f_row = tid >> 3, f_slot = tid & 7;
+        if constexpr (FULL) {  // (the keys of rows kPass apart are the same: one offset, and a base for every pass)
+            static_assert(kPass % 32 == 0, "keys");
+            src[0] = f_row * static_cast<uint32_t>(a.w_stride) + ((f_slot ^ key_w(f_row)) << 4);
+            src[1] = f_row * static_cast<uint32_t>(a.q_stride) + ((f_slot ^ key_q(f_row)) << 4);
+        } else
+#pragma unroll
+        for (int k = 0; k < kFetches; k++) {
+            const int at = k * kPass + f_row, t = at - kRows;
+            src[k] = k < kWeightFetches ? static_cast<uint32_t>(min(at, a.rows - 1 - r0)) * static_cast<uint32_t>(a.w_stride) + ((f_slot ^ key_w(at)) << 4)
+                                        : static_cast<uint32_t>(min(t, a.n_tokens - 1 - t0)) * static_cast<uint32_t>(a.q_stride) + ((f_slot ^ key_q(t)) << 4);
+        }
+        if constexpr (kTouch) {
+            // Lines of a later step into the L2: 32 compute units share it, `wide` of them a tile's weight rows and the others of a column its tokens;
+            // each asks for its part of both, four bytes a line, into LDS that nobody reads.
+            const int share_w = (kMine + wide - 1) / wide, per_w = (share_w + kWaves - 1) / kWaves, deep = 32 / wide, share_q = (kTokens + deep - 1) / deep, per_q = (share_q + kWaves - 1) / kWaves;
+            const int touch_w = row_share * share_w + wave * per_w + lane, touch_q = token_share % deep * share_q + wave * per_q + lane - per_w;
+            touches = lane < per_w + per_q;
+            const int8_t *w0 = weights(), *q0 = tokens();
+            touched = lane < per_w ? w0 + min(touch_w, min(kMine, a.rows - r0) - 1) * a.w_stride : q0 + min(max(touch_q, 0), min(kTokens, a.n_tokens - t0) - 1) * a.q_stride;
+        }
+    }
+    // First bytes of the tile's weight rows and tokens, in scalar registers.
+    __device__ __forceinline__ const int8_t *weights() const { return a.w + static_cast<int64_t>(__builtin_amdgcn_readfirstlane(r0)) * a.w_stride; }
+    __device__ __forceinline__ const int8_t *tokens() const { return a.q + static_cast<int64_t>(__builtin_amdgcn_readfirstlane(t0)) * a.q_stride; }
+    __device__ __forceinline__ void fetch(const int8_t *w0, const int8_t *q0, int k, int step, int stage) {
+        const uint32_t to = (lds0 + stage * kStage + k * (16 * kThreads) + wave * 1024);
+        const bool weight = k < kWeightFetches;
+        const int8_t *from = (weight ? w0 : q0) + step * KB;
+        if constexpr (FULL) from += static_cast<int64_t>(weight ? k : k - kWeightFetches) * kPass * (weight ? a.w_stride : a.q_stride);
+        const uint32_t off = src[FULL ? (weight ? 0 : 1) : k];
+        if (ONCE && weight) wide_dma16_once(to, wave_uniform(from), off);
+        else wide_dma16(to, wave_uniform(from), off);
+    }
+    __device__ __forceinline__ void touch(int step) {
+        if constexpr (kTouch) {
+            const int8_t *at = touched + step * KB;
+            asm volatile("s_mov_b32 m0, %0" ::"s"(__builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage + wave * 256)) : "memory", "m0");
+            if (touches) asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at) : "memory", "m0");
+        }
+    }
+    template <int SPLIT>
+    static constexpr bool fetched(int k) { return k >= kWeightFetches || k < kWeightFetches / SPLIT; }
+    template <int SPLIT>
+    static constexpr int fetches() { return kWeightFetches / SPLIT + kFetches - kWeightFetches; }
+    template <int SPLIT>
+    __device__ __forceinline__ void start() {
+        if (n_steps == 0) return;
+        const int8_t *w0 = weights(), *q0 = tokens();
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; k++)
+#pragma unroll
+            for (int f = 0; f < kFetches; f++)
+                if (fetched<SPLIT>(f)) fetch(w0, q0, f, min(k, n_steps - 1), k);
+        touch(min(STAGES, n_steps - 1));
+    }
+    // The last step where it is not whole: through registers, zeros behind the rows' ends.
+    template <int SPLIT>
+    __device__ __forceinline__ void fetch_rest(uint4 *smem) {
+        const int8_t *w0 = weights(), *q0 = tokens();
+#pragma unroll 1
+        for (int k = 0; k < kFetches; k++) {
+            if (!fetched<SPLIT>(k)) continue;
+            const int at = k * kPass + (tid >> 3), t = at - kRows;
+            const int piece = at < kRows ? (tid & 7) ^ key_w(at) : (tid & 7) ^ key_q(t);
+            const int8_t *p = at < kRows ? w0 + min(at, a.rows - 1 - r0) * a.w_stride : q0 + min(t, a.n_tokens - 1 - t0) * a.q_stride;
+            const int c = n_steps * KB + piece * 16;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (c + 16 <= a.cols) {
+                v = ldg16(p + c);
+            } else if (c < a.cols) {
+                uint32_t b[4] = {0, 0, 0, 0};
+                for (int j = 0; c + j < a.cols; j++) b[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[c + j])) << (8 * (j & 3));
+                v = make_uint4(b[0], b[1], b[2], b[3]);
+            }
+            smem[k * kThreads + tid] = v;
+        }
+    }
+
+    // Operands of a 32-value part of the step are read while the matrix cores work on the part before: two sets of registers, in turn.
+    template <int SPLIT>
+    __device__ __forceinline__ void read(int stage, int s) {
+        const int8_t *pa = lds + stage * kStage + ((at_a ^ (32 * s)) - wr * (MT - MT / SPLIT) * 32 * KB), *pb = lds + stage * kStage + (at_b ^ (32 * s));
+#pragma unroll
+        for (int i = 0; i < MT / SPLIT; i++) fa[s & 1][i] = *reinterpret_cast<const v4i_i8 *>(pa + i * 32 * KB);
+#pragma unroll
+        for (int j = 0; j < NT; j++) fb[s & 1][j] = *reinterpret_cast<const v4i_i8 *>(pb + j * 32 * KB);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // Requests go out one at a time between the matrix instructions (a wave that issues many in a row waits for the address unit): request f behind
+    // instruction f * span / fetches.
+    template <int SPLIT, bool FETCH>
+    __device__ __forceinline__ void multiply(const int8_t *w0, const int8_t *q0, int s, int step, int stage) {
+        constexpr int kN = fetches<SPLIT>(), kSlots = MT / SPLIT * NT * (kParts - 1), kSpan = kSlots < 2 * kN ? kSlots : 2 * kN;
+#pragma unroll
+        for (int i = 0; i < MT / SPLIT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[s & 1][i], fb[s & 1][j], acc[i][j], 0, 0, 0);
+                const int at = (s * (MT / SPLIT) + i) * NT + j;
+                if (FETCH && at < kSpan) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    int n = 0;
+#pragma unroll
+                    for (int f = 0; f < kFetches; f++)
+                        if (fetched<SPLIT>(f)) {
+                            if (n * kSpan / kN == at) fetch(w0, q0, f, step, stage);
+                            n++;
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // The sums of the tile that aim() and start() began.
+    template <int SPLIT>
+    __device__ __forceinline__ void sums(uint4 *smem) {
+        constexpr int kN = fetches<SPLIT>();
+        const int8_t *w0 = weights(), *q0 = tokens();
+#pragma unroll
+        for (int i = 0; i < MT / SPLIT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = v16i_i8{};
+        if (n_steps > 0) {
+            wide_wait<(STAGES - 2) * kN + kTouch>();
+            wide_barrier();
+            int stage = 0, into = STAGES - 1;  // the stage that was read last is filled next
+            read<SPLIT>(0, 0);
+            for (int step = 0; step < n_steps; step++) {
+                const int ahead = min(step + STAGES - 1, n_steps - 1);  // (past the end the last step again: the number of requests in flight stays the same)
+#pragma unroll
+                for (int s = 0; s + 1 < kParts; s++) {
+                    read<SPLIT>(stage, s + 1);
+                    multiply<SPLIT, true>(w0, q0, s, ahead, into);
+                }
+                touch(min(step + STAGES + 1, n_steps - 1));
+                into = stage;
+                stage = stage == STAGES - 1 ? 0 : stage + 1;
+                wide_wait<(STAGES - 2) * (kN + kTouch) + kTouch>();
+                wide_barrier();  // the next step is there for every wave, and every wave has read this one
+                read<SPLIT>(stage, 0);
+                multiply<SPLIT, false>(w0, q0, kParts - 1, 0, 0);
+            }
+            wide_wait<0>();
+        }
+        wide_barrier();  // (what was asked for past the end has come, for every wave: LDS is free)
+        if (a.cols % KB) {
+            fetch_rest<SPLIT>(smem);
+            wide_barrier();
+#pragma unroll
+            for (int s = 0; s < kParts; s++) {
+                read<SPLIT>(0, s);
+                multiply<SPLIT, false>(w0, q0, s, 0, 0);
+            }
+            wide_barrier();
+        }
+    }
+    // A lane has 16 neighbouring rows of one token: stored so, a wave would write 16 bytes here and there (256 x 256 cells 10 us).  They change places in LDS, each
+    // wave's in its own 8 KB of the second stage, 32 tokens by up to 256 bytes at a time, and leave as whole runs.  Slots are exclusive-ored here too.
+    template <int SPLIT>
+    __device__ __forceinline__ void store(uint4 *smem, int row, int token) {
+        row = __builtin_amdgcn_readfirstlane(row);
+        token = __builtin_amdgcn_readfirstlane(token);
+        typedef typename T::Bits Bits;
+        // (what follows depends on this copy: otherwise its addresses are kept in registers through the sums of every tile)
+        int lane = this->lane;
+        asm volatile("" : "+v"(lane));
+        const int m = lane & 31, half = lane >> 5;
+        constexpr int kMine = MT / SPLIT, kPhase = kMine * 32 * static_cast<int>(sizeof(Bits)) > 256 ? 8 / static_cast<int>(sizeof(Bits)) : kMine;  // row tiles at a time
+        constexpr int kSlots = kPhase * 32 * static_cast<int>(sizeof(Bits)) / 16, kPer = 16 / static_cast<int>(sizeof(Bits));
+        static_assert(STAGES * kStage - kStage >= kWaves * 32 * kSlots * 16, "LDS behind the first stage");
+        uint4 *mine = smem + kStage / 16 + wave * (32 * kSlots);
+        float *scales = reinterpret_cast<float *>(smem + kScales / 16);
+        for (int r = tid; r < kRows / SPLIT; r += kThreads) {
+            scales[r] = a.w_scales[min(row + r, a.rows - 1)];
+            scales[kRows + r] = a.bias ? a.bias[min(row + r, a.rows - 1)] : 0.0f;
+        }
+        wide_barrier();
+        auto swap = [](int t, int slot) { return t * kSlots + (slot ^ (kSlots == 16 ? t & 15 : kSlots == 8 ? t >> 1 & 7 : t >> 2 & 3)); };
+#pragma unroll
+        for (int i0 = 0; i0 < kMine; i0 += kPhase) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int t0 = token + (wt * NT + j) * 32;
+                const float s = a.scales[FULL ? t0 + m : min(t0 + m, a.n_tokens - 1)];
+#pragma unroll
+                for (int i = 0; i < kPhase; i++) {
+                    const int r = (wr * kMine + i0 + i) * 32 + 16 * half;
+                    float v[16];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float4 f = *reinterpret_cast<const float4 *>(scales + r + 4 * k);
+                        v[4 * k] = static_cast<float>(acc[i0 + i][j][4 * k]) * s * f.x;
+                        v[4 * k + 1] = static_cast<float>(acc[i0 + i][j][4 * k + 1]) * s * f.y;
+                        v[4 * k + 2] = static_cast<float>(acc[i0 + i][j][4 * k + 2]) * s * f.z;
+                        v[4 * k + 3] = static_cast<float>(acc[i0 + i][j][4 * k + 3]) * s * f.w;
+                    }
+                    if (a.bias)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float4 f = *reinterpret_cast<const float4 *>(scales + kRows + r + 4 * k);
+                            v[4 * k] = v[4 * k] + f.x;
+                            v[4 * k + 1] = v[4 * k + 1] + f.y;
+                            v[4 * k + 2] = v[4 * k + 2] + f.z;
+                            v[4 * k + 3] = v[4 * k + 3] + f.w;
+                        }
+#pragma unroll
+                    for (int k = 0; k < 16 / kPer; k++) {
+                        uint4 packed;
+                        if constexpr (sizeof(Bits) == 4)
+                            packed = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3]));
+                        else
+                            packed = make_uint4(T::narrow(v[8 * k]) | T::narrow(v[8 * k + 1]) << 16, T::narrow(v[8 * k + 2]) | T::narrow(v[8 * k + 3]) << 16,
+                                                T::narrow(v[8 * k + 4]) | T::narrow(v[8 * k + 5]) << 16, T::narrow(v[8 * k + 6]) | T::narrow(v[8 * k + 7]) << 16);
+                        mine[swap(m, (2 * i + half) * (16 / kPer) + k)] = packed;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const int r = row + (wr * kMine + i0) * 32;
+#pragma unroll
+                for (int q = 0; q < kSlots / 2; q++) {
+                    const int at = q * 64 + lane, t = at / kSlots, slot = at % kSlots, rr = r + slot * kPer;
+                    const uint4 v = mine[swap(t, slot)];
+                    if (!FULL && (t0 + t >= a.n_tokens || rr >= a.rows)) continue;
+                    Bits *out = static_cast<Bits *>(a.out) + (t0 + t) * a.out_stride + rr;
+                    if (FULL || rr + kPer <= a.rows) {
+                        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
+                        *reinterpret_cast<v4u *>(out) = v4u{v.x, v.y, v.z, v.w};
+                    } else {
+                        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < kPer; e++)
+                            if (rr + e < a.rows) out[e] = sizeof(Bits) == 4 ? __builtin_bit_cast(Bits, static_cast<std::conditional_t<sizeof(Bits) == 4, uint32_t, uint16_t>>(word[e])) : __builtin_bit_cast(Bits, static_cast<std::conditional_t<sizeof(Bits) == 4, uint32_t, uint16_t>>(word[e / 2] >> (16 * (e & 1))));
+                    }
+                }
+            }
+        }
+    }
+};
+
+// A workgroup a tile.
+template <class T, int WR, int WT, int MT, int NT, int STAGES, int PER_CU, bool ONCE>
+__global__ __launch_bounds__(64 * WR * WT, WR * WT * PER_CU / 4) void matmul_i8_tile_kernel(MatmulI8 a, TileGrid grid) {
+    extern __shared__ uint4 smem[];
+    TileWork<T, WR, WT, MT, NT, STAGES, ONCE, false> work(a, smem);
+    const int total = grid.n_row_blocks * grid.n_token_blocks, per = total >> 3, more = total & 7, xcd = blockIdx.x & 7;
+    int row_block, token_block, wide;
+    tile_of(grid, xcd * per + min(xcd, more) + (blockIdx.x >> 3), row_block, token_block, wide);
+    const int row = row_block * work.kRows, token = token_block * work.kTokens;
+    work.template aim<1>(row, token, token_block % wide, wide, row_block);
+    work.template start<1>();
+    work.template sums<1>(smem);
+    work.template store<1>(smem, row, token);
+}
+
+// A workgroup a compute unit, 32 an XCD: each walks the tiles of its XCD's run 32 apart, and asks for the next tile's first step before it stores the one
+// it has.  The tiles that are left when all 32 can no longer have a whole one are cut into halves or quarters of their rows where that gives every
+// unit some (896 tiles, 4096 tokens on 14336 rows: the time of 3.5 tiles instead of 4).  The last tiles of a side that is no whole number of them reach back
+// into their neighbours: cells that two workgroups write get the same bits.
+template <class T, int WR, int WT, int MT, int NT>
+__global__ __launch_bounds__(64 * WR * WT, WR * WT / 4) void matmul_i8_walk_kernel(MatmulI8 a, TileGrid grid) {
+    extern __shared__ uint4 smem[];
+    TileWork<T, WR, WT, MT, NT, 2, false, true> work(a, smem);
+    constexpr int kRows = work.kRows, kTokens = work.kTokens;
+    const int total = grid.n_row_blocks * grid.n_token_blocks, per = total >> 3, more = total & 7, xcd = blockIdx.x & 7, unit = blockIdx.x >> 3;
+    const int first = xcd * per + min(xcd, more), n = per + (xcd < more ? 1 : 0);
+    const int rounds = n >> 5, left = n & 31, split = left == 0 || left > 16 ? 1 : left > 8 ? 2 : 4;
+    // This unit's items: whole tiles and at most one part.  Every other unit takes its part first, so that not all of them come to their stores at the
+    // same time.
+    const bool part = split > 1 && unit < left * split, part_first = part && (unit & 1) != 0;
+    const int wholes = rounds + (split == 1 && unit < left ? 1 : 0), items = wholes + (part ? 1 : 0);
+    int row = 0, token = 0;
+    auto is_part = [&](int item) __attribute__((always_inline)) { return part && item == (part_first ? 0 : wholes); };
+    auto begin = [&](int item) __attribute__((always_inline)) {
+        int row_block, token_block, wide;
+        if (!is_part(item)) {
+            tile_of(grid, first + (item - (part_first ? 1 : 0)) * 32 + unit, row_block, token_block, wide);
+            row = min(row_block * kRows, a.rows - kRows);
+            token = min(token_block * kTokens, a.n_tokens - kTokens);
+            work.template aim<1>(row, token, token_block % wide, wide, row_block);
+            work.template start<1>();
+        } else {
+            tile_of(grid, first + rounds * 32 + unit / split, row_block, token_block, wide);
+            row = min(row_block * kRows, a.rows - kRows) + unit % split * (kRows / split);
+            token = min(token_block * kTokens, a.n_tokens - kTokens);
+            if (split == 2) {
+                work.template aim<2>(row, token, 0, 1, 0);
+                work.template start<2>();
+            } else {
+                work.template aim<4>(row, token, 0, 1, 0);
+                work.template start<4>();
+            }
+        }
+    };
+    if (items > 0) begin(0);
+#pragma unroll 1
+    for (int item = 0; item < items; item++) {
+        const int cut = is_part(item) ? split : 1, r = row, t = token;
+        auto run = [&](auto parts) __attribute__((always_inline)) {
+            constexpr int kParts = decltype(parts)::value;
+            work.template sums<kParts>(smem);
+            if (item + 1 < items) begin(item + 1);
+            work.template store<kParts>(smem, r, t);
+        };
+        if (cut == 1) run(std::integral_constant<int, 1>{});
+        else if (cut == 2) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, 4>{});
+    }
+}
+
+template <class K>
+static int allow_lds(K kernel, size_t bytes, std::atomic<bool> &raised) {
+    if (bytes > 64 * 1024 && !raised.load(std::memory_order_acquire)) {  // (a launch may use that much without asking)
+        CML_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+        raised.store(true, std::memory_order_release);
+    }
+    return CML_OK;
+}
+
+inline TileGrid tile_grid(const MatmulI8 &a, int rows, int tokens) {
+    const int n = (a.n_tokens + tokens - 1) / tokens;
+    return TileGrid{(a.rows + rows - 1) / rows, n, std::min(4, n)};
+}
+
+template <class T, int WR, int WT, int MT, int NT, int STAGES, int PER_CU, bool ONCE = false>
+static int launch_tile(const MatmulI8 &a, hipStream_t st) {
+    typedef TileWork<T, WR, WT, MT, NT, STAGES, ONCE, false> Work;
+    static_assert(Work::kLds * PER_CU <= 160 * 1024, "LDS");
+    const auto kernel = matmul_i8_tile_kernel<T, WR, WT, MT, NT, STAGES, PER_CU, ONCE>;
+    static std::atomic<bool> raised{false};
+    if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
+    const TileGrid grid = tile_grid(a, Work::kRows, Work::kTokens);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid.n_row_blocks * grid.n_token_blocks)), dim3(Work::kThreads), Work::kLds, st, a, grid);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+
+template <class T>
+static int launch_walk(const MatmulI8 &a, hipStream_t st) {
+    typedef TileWork<T, 2, 4, 4, 2, 2, false, true> Work;
+    const auto kernel = matmul_i8_walk_kernel<T, 2, 4, 4, 2>;
+    static std::atomic<bool> raised{false};
+    if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(256), dim3(Work::kThreads), Work::kLds, st, a, tile_grid(a, Work::kRows, Work::kTokens));
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+
+// What a call takes by tile, in microseconds: a start of 3, then per workgroup that a compute unit runs `work` for each step of 128 values and `ends` for the tile;
+// no tile is through its steps faster than `step` each, alone on its unit.  Fitted to 1 - 4096 tokens on nine weight shapes (704 x 2816 to 128256 x 2048):
+// the tile that it picks takes 0.8 % more than the best one in the mean, 13 % at most.
+struct TileCost {
+    int rows, tokens, per_unit;
+    float step, work, ends;
+};
+constexpr TileCost kWalk{256, 256, 1, 1.12f, 0.85f, 6.2f}, kTiles[] = {{256, 128, 1, 0.73f, 0.63f, 3.2f}, {128, 128, 1, 0.51f, 0.435f, 2.9f}, {64, 128, 2, 0.36f, 0.32f, 0.92f},
+                                                                       {64, 64, 2, 0.236f, 0.213f, 0.5f}, {64, 32, 3, 0.213f, 0.174f, 0.4f}};
+static float tile_cost(const MatmulI8 &a, const TileCost &c) {
+    const int64_t tiles = static_cast<int64_t>((a.rows + c.rows - 1) / c.rows) * ((a.n_tokens + c.tokens - 1) / c.tokens);
+    const float steps = static_cast<float>((a.cols + 127) / 128), one = c.work * steps + c.ends;
+    if (&c == &kWalk) return 3.0f + std::max(c.step * steps, std::max(1.0f, 0.5f * static_cast<float>((tiles + 127) / 128)) * one);  // (half rounds)
+    const int64_t full = tiles / (256 * c.per_unit), left = tiles - full * 256 * c.per_unit;
+    return 3.0f + static_cast<float>(full * c.per_unit) * one + (left ? std::max(c.step * steps, static_cast<float>((left + 255) / 256) * one) : 0.0f);
+}
+
+// Variants: 0 the walk, 1 - 5 kTiles, 6 / 7 tiles of 128 x 64 / 64 x 64 that ask for the weight past the caches, 8 / 9 few tokens with eight / four waves.
+static int choose_variant(const MatmulI8 &a) {
+    const int64_t bytes = static_cast<int64_t>(a.rows) * a.cols;
+    // A weight of 96 MB and more is used once in a pass over a model: past the caches (128256 x 2048, 1 / 16 / 37 tokens: 52 / 55 / 59 us plain, 45 / 46 / 49 so), in the
+    // tile that has two workgroups for every compute unit (32000 x 4096, 1 / 32 tokens: 128 x 64 31 / 29, 64 x 64 29 / 28; 48 tokens: 30 / 30, plain 24).
+    if (bytes >= 96ll << 20 && a.n_tokens <= 64) {
+        if ((a.rows + 127) / 128 >= 512) return 6;
+        if (a.n_tokens <= 32) return 7;
+    }
+    int best = 1;
+    float least = tile_cost(a, kTiles[0]);
+    for (int i = 1; i < 5; i++) {
+        const float c = tile_cost(a, kTiles[i]);
+        if (c < least) {
+            least = c;
+            best = i + 1;
+        }
+    }
+    if (a.rows >= 256 && a.n_tokens >= 256 && tile_cost(a, kWalk) < least) return 0;
+    // Few tokens: no steps to wait for, but every workgroup reads the tokens for itself (4096 x 14336, 1 / 16 tokens: 13.9 / 18.3 us, tiles 30 / 31; 14336 x 4096: 15.0 / 20.0
+    // and 15.3 / 15.8).  Four waves from 8192 rows (8192 x 1024: 4.3 us, eight 4.4; 128256 x 2048: 48 and 61).
+    if (a.n_tokens <= 16 && 3.0f + (0.17f + 0.0055f * static_cast<float>(a.n_tokens)) * 1e-6f * static_cast<float>(bytes) < least) return a.rows < 8192 ? 8 : 9;
+    return best;
+}
+
+template <class T>
+static int launch_variant(int v, const MatmulI8 &a, hipStream_t st) {
+    switch (v) {
+        case 0: return launch_walk<T>(a, st);
+        case 1: return launch_tile<T, 4, 2, 2, 2, 3, 1>(a, st);
+        case 2: return launch_tile<T, 2, 2, 2, 2, 4, 1>(a, st);
+        case 3: return launch_tile<T, 2, 4, 1, 1, 3, 2>(a, st);
+        case 4: return launch_tile<T, 2, 2, 1, 1, 4, 2>(a, st);
+        case 5: return launch_tile<T, 2, 1, 1, 1, 4, 3>(a, st);
+        case 6: return launch_tile<T, 4, 1, 1, 2, 3, 2, true>(a, st);
+        case 7: return launch_tile<T, 2, 2, 1, 1, 4, 2, true>(a, st);
+        case 8: return launch_few<T, 8>(a, st);
+        default: return launch_few<T, 4>(a, st);
+    }
+}
+
 int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int64_t n_tokens, const int8_t *w, int64_t w_stride, const float *w_scales, int64_t rows, int64_t cols,
                      const float *bias, int dtype, void *out, int64_t out_stride, hipStream_t st) {
     const MatmulI8 a{q, w, scales, w_scales, bias, out, q_stride, w_stride, out_stride, static_cast<int>(n_tokens), static_cast<int>(rows), static_cast<int>(cols)};
+    const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(w) | static_cast<uintptr_t>(q_stride | w_stride)) & 15u) == 0 &&
+                         q_stride < (1 << 23) && w_stride < (1 << 23);  // (256 rows within 32 bits)
+    const int forced = env_int("CAMELID_HIP_I8_TILE", 0);  // n: variant n - 1 where it serves the call; -1: staged
+    int v = choose_variant(a);
+    if (forced > 0 && forced <= 10 && !(forced == 1 && (rows < 256 || n_tokens < 256)) && !(forced >= 9 && n_tokens > 16)) v = forced - 1;
+    if (!aligned && v < 8 && n_tokens <= 16 && forced >= 0) v = rows < 8192 ? 8 : 9;
+    if (forced >= 0 && (aligned || v >= 8)) {
+        switch (v) {
+            case 0: CML_COUNT_LAUNCH("i8.matmul.walk"); break;
+            case 8: case 9: CML_COUNT_LAUNCH("i8.matmul.few"); break;
+            case 6: case 7: CML_COUNT_LAUNCH("i8.matmul.tile.once"); break;
+            default: CML_COUNT_LAUNCH("i8.matmul.tile"); break;
+        }
+        return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
+    }
     CML_COUNT_LAUNCH("i8.matmul.staged");
     return with_type(dtype, [&](auto t) {
         const dim3 grid(static_cast<unsigned>((rows + 63) / 64), static_cast<unsigned>((n_tokens + 63) / 64));
