@@ -3,12 +3,12 @@
 //   m = max x, S = sum exp(x - m), H = ln S - sum exp(x - m) (x - m) / S,  log p(t) = (x_t - m) - ln S
 //   rank(t) = 1 + the tokens with a larger logit, or the same and a lower index
 //
-// A row is cut into parts, one wave each; a wave reads its part once, in batches of kBatch neighbouring logits, and keeps per lane the running maximum
-// and the two sums, and across its lanes the sorted list of the best (lane i: the i-th).  Parts of a row are joined by a second launch.
+// A row is cut into parts, one wave each; a wave reads its part once, in batches of neighbouring logits (the next one requested before this one is looked
+// at), and keeps per lane the running maximum and the two sums, and across its lanes the sorted list of the best (lane i: the i-th).  Parts of a
+// row are joined inside the workgroup where it has them all, else by a second launch.
 //
-// A logit is looked at for the list only where a batch holds one above the list's last; candidates enter in the order of their index,
-// so a strict comparison leaves ties with the lower index.  Where a batch holds many (the first one; ascending logits), a bisection over the
-// lanes' maxima first finds a value that at least n of the batch reach.
+// Logits are looked at one by one for the list only where a batch holds one above the list's last.  Where it holds many (the first one; ascending
+// logits), a bisection over the lanes' maxima first finds a value that at least n of the batch reach.
 //
 // -inf is a masked token: probability 0, no alternative.  A row of nothing else has log probability -inf, entropy 0 and no alternatives.  NaN or +inf in a
 // row leaves NaN in log probability and entropy, as the formula does.  A row at the type's lowest value is an ordinary, uniform row.
@@ -22,8 +22,7 @@ namespace cml {
 
 constexpr float kLowest = -3.4028235e38f;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
-constexpr int kBatch = 1024;      // logits a wave takes at once: 16 a lane
-constexpr int kMaxParts = 128;    // per row
+constexpr int kMaxParts = 128;  // per row: two for a lane of the joining wave
 
 struct ScoreArgs {
     const void *logits;
@@ -35,7 +34,8 @@ struct ScoreArgs {
     int vocab, n_top, parts;
 };
 
-__host__ __device__ constexpr int partial_floats(int n_top) { return 4 + 2 * n_top; }
+// most, sum, esum, above, the given logit; the list's values, its ids
+__host__ __device__ constexpr int partial_floats(int n_top) { return 5 + 2 * n_top; }
 
 // What a wave has seen of a row.  Per lane: most, sum, esum; the same in all lanes: above.
 struct RowState {
@@ -43,21 +43,28 @@ struct RowState {
     float sum = 0.0f;       // of exp(x - most)
     float esum = 0.0f;      // of exp(x - most) (x - most) log2(e)
     int above = 0;          // tokens ahead of the given one
-    float list = -INFINITY; // lane i: the i-th best
-    int list_id = -1;
+    uint32_t list = 0, list_low = 0;  // lane i: the i-th best, by the value's ordered bits, then the inverted id; 0: none
 };
 
 // d as a factor: the exponential of one so low is 0, and 0 times a finite number adds nothing (a masked token, an overflowed difference).
 __device__ __forceinline__ float finite_factor(float d) { return fmaxf(d, -1e25f); }
 
-__device__ __forceinline__ void list_insert(RowState &s, float v, int id, int lane) {
-    const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(s.list >= v));
-    const float up = dpp_f32<0x138>(s.list);  // wave_shr:1
-    const int up_id = __builtin_amdgcn_update_dpp(0, s.list_id, 0x138, 0xf, 0xf, false);
-    s.list = lane < at ? s.list : lane == at ? v : up;
-    s.list_id = lane < at ? s.list_id : lane == at ? id : up_id;
+// A finite or infinite f32 as an unsigned integer that orders like it (-0 as 0), above 0, and back.
+__device__ __forceinline__ uint32_t ordered(uint32_t bits) {
+    bits = bits == 0x80000000u ? 0u : bits;
+    return bits ^ (static_cast<uint32_t>(static_cast<int>(bits) >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float from_ordered(uint32_t v) { return v == 0 ? -INFINITY : __uint_as_float(v & 0x80000000u ? v ^ 0x80000000u : ~v); }
 
+// Into its place by value, then by id; what falls off lane 63 is gone.  Every lane decides for itself, from its entry and the one before it.  (What an
+// insertion takes is its instructions: 20 in front of every list of 20, 60 to 100 a part.)
+__device__ __forceinline__ void list_insert(RowState &s, uint32_t v, int id) {
+    const uint64_t c = static_cast<uint64_t>(v) << 32 | static_cast<uint32_t>(~id), mine = static_cast<uint64_t>(s.list) << 32 | s.list_low;
+    const uint32_t up = __builtin_amdgcn_update_dpp(-1, s.list, 0x138, 0xf, 0xf, false), up_low = __builtin_amdgcn_update_dpp(-1, s.list_low, 0x138, 0xf, 0xf, false);  // wave_shr:1, all ones in lane 0
+    const bool stays = mine > c, after = (static_cast<uint64_t>(up) << 32 | up_low) > c;
+    s.list = stays ? s.list : after ? v : up;
+    s.list_low = stays ? s.list_low : after ? static_cast<uint32_t>(~id) : up_low;
+}
 // The running sums of a lane moved to another maximum.
 __device__ __forceinline__ void rebase(RowState &s, float most) {
     const float d = (s.most - most) * kLog2e, f = __builtin_amdgcn_exp2f(d);
@@ -66,13 +73,25 @@ __device__ __forceinline__ void rebase(RowState &s, float most) {
     s.most = most;
 }
 
-// A value that at least n of the 64 lanes' v reach, close to the n-th largest: bisection over the upper half of the ordered bits.
-__device__ __forceinline__ float nth_bound(float v, int n) {
-    const int key = total_key(v) >> 16;
-    int low = -32768;
-    for (int bit = 32768; bit; bit >>= 1)
-        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(key >= low + bit)) >= n) low += bit;
-    return from_total_key(static_cast<int>(static_cast<unsigned>(low) << 16));
+// A value that at least n of the 64 K values v are above, close below the n-th largest: bisection over the upper half of the ordered bits.  Where hardly more than
+// n are above `over`, that.
+template <int K>
+__device__ __forceinline__ float below_nth(const float (&v)[K], int n, float over) {
+    int above = 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[k] > over));
+    if (above <= n + 8) return over;  // (the search takes what eight insertions do)
+    int key[K], low = -32768;
+#pragma unroll
+    for (int k = 0; k < K; k++) key[k] = total_key(v[k]) >> 16;
+    for (int bit = 32768; bit; bit >>= 1) {
+        int reach = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] >= low + bit));
+        if (reach >= n) low += bit;
+    }
+    const int under = static_cast<int>(static_cast<unsigned>(low) << 16) - 1;
+    return fmaxf(over, from_total_key(under == -1 ? -2 : under));  // (-0 is not below 0)
 }
 
 // Sums over the lanes, every lane at the row's maximum.
@@ -92,155 +111,261 @@ __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, const
         if (a.entropy) a.entropy[row] = empty ? 0.0f : log_sum - s.esum / s.sum * kLn2;
     }
     if (lane < a.n_top) {
-        a.top_ids[row * a.n_top + lane] = s.list_id;
-        a.top_log_probs[row * a.n_top + lane] = s.list_id < 0 ? -INFINITY : (s.list - s.most) - log_sum;
+        a.top_ids[row * a.n_top + lane] = s.list ? static_cast<int>(~s.list_low) : -1;
+        a.top_log_probs[row * a.n_top + lane] = s.list ? (from_ordered(s.list) - s.most) - log_sum : -INFINITY;
     }
 }
 
+// A lane's logits of a batch: pieces of eight, 64 lanes apart.
 template <class T>
+struct Batch {
+    static constexpr int kPieces = sizeof(typename T::Bits) == 4 ? 2 : 4, kLogits = 64 * 8 * kPieces;
+    v4u_row raw[kPieces * (sizeof(typename T::Bits) == 4 ? 2 : 1)];
+
+    __device__ __forceinline__ void request(const typename T::Bits *p) {  // p: the lane's first logit
+        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
+        constexpr int kPer = sizeof(typename T::Bits) == 4 ? 2 : 1;
+#pragma unroll
+        for (int u = 0; u < kPieces; u++)
+#pragma unroll
+            for (int k = 0; k < kPer; k++) raw[u * kPer + k] = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(p + u * 512) + k);
+    }
+    __device__ __forceinline__ void take(float (&v)[kPieces][8]) const {
+#pragma unroll
+        for (int u = 0; u < kPieces; u++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if constexpr (sizeof(typename T::Bits) == 4) v[u][j] = __uint_as_float(raw[2 * u + j / 4][j % 4]);
+                else v[u][j] = T::widen(j & 1 ? raw[u][j / 2] >> 16 : raw[u][j / 2] & 0xffffu);
+            }
+    }
+};
+
+// INSIDE: 1, 2 or 4 parts a row, all of them in one workgroup.
+template <class T, bool INSIDE>
 __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
     typedef typename T::Bits Bits;
-    constexpr int EP = 8, U = kBatch / 64 / EP;  // a piece of eight logits a lane
+    constexpr int U = Batch<T>::kPieces, kBatch = Batch<T>::kLogits;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-    const int64_t row = id / a.parts;
-    const int part = static_cast<int>(id - row * a.parts);
-    if (row >= a.n_rows) return;
-    const Bits *x = static_cast<const Bits *>(a.logits) + row * a.stride;
-    const int target = a.target[row];
+    const uint32_t id = blockIdx.x * 4 + wave, row = id / static_cast<uint32_t>(a.parts), part = id - row * a.parts;
+    const bool live = row < a.n_rows;
+    if (!live && !INSIDE) return;
+    const Bits *x = static_cast<const Bits *>(a.logits) + (live ? row : 0) * a.stride;
+    const int n_batches = (a.vocab + kBatch - 1) / kBatch;
+    const int begin = static_cast<int>(static_cast<int64_t>(n_batches) * part / a.parts), end = live ? static_cast<int>(static_cast<int64_t>(n_batches) * (part + 1) / a.parts) : 0;
+    Batch<T> ahead;
+    const Bits *mine = x + lane * 8;
+    if (begin < end && (begin + 1) * kBatch <= a.vocab) ahead.request(mine + begin * kBatch);
+    const int target = live ? a.target[row] : -1;
     const bool in_range = target >= 0 && target < a.vocab;
     const float given = in_range ? load_value<T>(x + target) : INFINITY;
-    const int n_batches = (a.vocab + kBatch - 1) / kBatch;
-    const int begin = static_cast<int>(static_cast<int64_t>(n_batches) * part / a.parts), end = static_cast<int>(static_cast<int64_t>(n_batches) * (part + 1) / a.parts);
     RowState s;
     float last = -INFINITY;  // the list's n-th
+#pragma unroll 1
     for (int b = begin; b < end; b++) {
         const int base = b * kBatch;
-        float v[U][EP];
+        const bool whole = base + kBatch <= a.vocab;
+        float v[U][8];
+        // vmcnt(0): the batch is here.  Said outright, because the compiler, which does not see that no path leaves it in flight, otherwise waits below, at
+        // reused registers, for the next batch as well (512 x 128256 bf16 63 us).
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        if (whole) {
+            ahead.take(v);
+            if (b + 1 < end && base + 2 * kBatch <= a.vocab) ahead.request(mine + base + kBatch);
+        } else {  // the row's last batch
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int i = base + (u * 64 + lane) * 8 + j;
+                    v[u][j] = i < a.vocab ? load_value<T>(x + i) : -INFINITY;
+                }
+        }
+        float pm[U], bm = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int i = base + (u * 64 + lane) * EP;
-            if (i + EP <= a.vocab) {
-                load8<T>(x + i, v[u]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < EP; j++) v[u][j] = i + j < a.vocab ? load_value<T>(x + i + j) : -INFINITY;
-            }
+            pm[u] = fmaxf(fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3])), fmaxf(fmaxf(v[u][4], v[u][5]), fmaxf(v[u][6], v[u][7])));
+            bm = fmaxf(bm, pm[u]);
         }
-        float bm = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < EP; j++) bm = fmaxf(bm, v[u][j]);
         rebase(s, fmaxf(s.most, bm));
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int j = 0; j < EP; j++) {
+            for (int j = 0; j < 8; j++) {
                 const float d = (v[u][j] - s.most) * kLog2e, e = __builtin_amdgcn_exp2f(d);
                 s.sum = s.sum + e;
                 s.esum = fmaf(e, finite_factor(d), s.esum);
-                const int i = base + (u * 64 + lane) * EP + j;
-                s.above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < a.vocab && (v[u][j] > given || (v[u][j] == given && i < target))));
             }
+        // tokens ahead of the given one: of equal logits those with a lower index
+        if (whole && base + kBatch <= target) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) s.above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[u][j] >= given));
+        } else if (whole && base > target) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) s.above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[u][j] > given));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int i = base + (u * 64 + lane) * 8 + j;
+                    s.above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < a.vocab && (v[u][j] > given || (v[u][j] == given && i < target))));
+                }
+        }
         if (a.n_top == 0) continue;
-        unsigned long long lanes = __builtin_amdgcn_ballot_w64(bm > last);
-        if (!lanes) continue;
-        float bound = -INFINITY;
-        if (__builtin_popcountll(lanes) > a.n_top) bound = nth_bound(bm, a.n_top);
+        if (!__builtin_amdgcn_ballot_w64(bm > last)) continue;
+        // (what the list holds has lower indices than this batch: only larger logits get in)
+        const float most[1] = {bm};
+        const float over = below_nth(most, a.n_top, last);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            float pm = v[u][0];
+            if (!__builtin_amdgcn_ballot_w64(pm[u] > over)) continue;
 #pragma unroll
-            for (int j = 1; j < EP; j++) pm = fmaxf(pm, v[u][j]);
-            lanes = __builtin_amdgcn_ballot_w64(pm > last && pm >= bound);
-            while (lanes) {
-                const int from = __builtin_ctzll(lanes);
-                lanes &= lanes - 1;
-#pragma unroll
-                for (int j = 0; j < EP; j++) {
-                    const float c = lane_of(v[u][j], from);
-                    if (c > last && c >= bound) {
-                        list_insert(s, c, base + (u * 64 + from) * EP + j, lane);
-                        last = lane_of(s.list, a.n_top - 1);
-                    }
+            for (int j = 0; j < 8; j++) {
+                unsigned long long in = __builtin_amdgcn_ballot_w64(v[u][j] > over);
+                while (in) {
+                    const int from = __builtin_ctzll(in);
+                    in &= in - 1;
+                    list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[u][j]), from)), base + (u * 64 + from) * 8 + j);
                 }
             }
         }
+        last = from_ordered(__builtin_amdgcn_readlane(s.list, a.n_top - 1));
     }
     close(s);
-    if (a.parts == 1) {
+    if constexpr (INSIDE) {
+        __shared__ float sums[4][3];
+        __shared__ int aboves[4];
+        __shared__ uint2 lists[4][64];
+        if (part > 0) {
+            if (lane == 0) {
+                sums[wave][0] = s.most;
+                sums[wave][1] = s.sum;
+                sums[wave][2] = s.esum;
+                aboves[wave] = s.above;
+            }
+            lists[wave][lane] = make_uint2(s.list, s.list_low);
+        }
+        __syncthreads();
+        if (part > 0 || !live) return;
+        for (int p = wave + 1; p < wave + a.parts; p++) {
+            RowState o;
+            o.most = sums[p][0];
+            o.sum = sums[p][1];
+            o.esum = sums[p][2];
+            const float most = fmaxf(s.most, o.most);
+            rebase(s, most);
+            rebase(o, most);
+            s.sum = s.sum + o.sum;
+            s.esum = s.esum + o.esum;
+            s.above += aboves[p];
+            if (a.n_top == 0) continue;
+            const uint2 theirs = lists[p][lane];
+            // (of equal logits those of this list have the lower ids)
+            unsigned long long in = __builtin_amdgcn_ballot_w64(theirs.x > static_cast<uint32_t>(__builtin_amdgcn_readlane(s.list, a.n_top - 1)));
+            while (in) {
+                const int from = __builtin_ctzll(in);
+                in &= in - 1;
+                list_insert(s, __builtin_amdgcn_readlane(theirs.x, from), ~__builtin_amdgcn_readlane(theirs.y, from));
+            }
+        }
         write_row<T>(a, row, s, given, in_range, lane);
     } else {
-        float *p = a.partial + id * partial_floats(a.n_top);
+        float *p = a.partial + static_cast<int64_t>(id) * partial_floats(a.n_top);
         if (lane == 0) {
             p[0] = s.most;
             p[1] = s.sum;
             p[2] = s.esum;
             p[3] = __builtin_bit_cast(float, s.above);
+            p[4] = given;
         }
         if (lane < a.n_top) {
-            p[4 + lane] = s.list;
-            p[4 + a.n_top + lane] = __builtin_bit_cast(float, s.list_id);
+            p[5 + lane] = from_ordered(s.list);
+            p[5 + a.n_top + lane] = __uint_as_float(~s.list_low);
         }
     }
 }
 
-// The parts of a row, joined by one wave: lane p takes the sums of parts p, p + 64, ...; the lists go in order.
+// The parts of a row, joined by one wave, lane p taking parts p and p + 64.  Of the lists only what reaches the n-th largest of the parts' best is looked at.
 template <class T>
 __global__ __launch_bounds__(64) void token_log_probs_join_kernel(ScoreArgs a) {
-    typedef typename T::Bits Bits;
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
     const int width = partial_floats(a.n_top);
-    const float *p = a.partial + row * a.parts * width;
+    const float *rows = a.partial + row * a.parts * width;
+    const int target = a.target[row];
+    const bool in_range = target >= 0 && target < a.vocab;
+    const float given = rows[4];
     RowState s;
-    for (int i = lane; i < a.parts; i += 64) {
+    float best[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const bool here = lane + 64 * k < a.parts;
+        const float *p = rows + min(lane + 64 * k, a.parts - 1) * width;
         RowState o;
-        o.most = p[i * width];
-        o.sum = p[i * width + 1];
-        o.esum = p[i * width + 2];
+        o.most = here ? p[0] : kLowest;
+        o.sum = here ? p[1] : 0.0f;
+        o.esum = here ? p[2] : 0.0f;
+        best[k] = here && a.n_top ? p[5] : -INFINITY;
         const float most = fmaxf(s.most, o.most);
         rebase(s, most);
         rebase(o, most);
         s.sum = s.sum + o.sum;
         s.esum = s.esum + o.esum;
-        s.above += __builtin_bit_cast(int, p[i * width + 3]);
+        s.above += here ? __builtin_bit_cast(int, p[3]) : 0;
     }
     close(s);
+#pragma unroll
     for (int o = 1; o < 64; o <<= 1) s.above += __shfl_xor(s.above, o);
-    float last = -INFINITY;
-    const int n = a.parts * a.n_top;
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = min(i0 + lane, n - 1), part = i / a.n_top, at = i - part * a.n_top;
-        const float v = i0 + lane < n ? p[part * width + 4 + at] : -INFINITY;
-        const int id = __builtin_bit_cast(int, p[part * width + 4 + a.n_top + at]);
-        unsigned long long lanes = __builtin_amdgcn_ballot_w64(v > last);
-        while (lanes) {
-            const int from = __builtin_ctzll(lanes);
-            lanes &= lanes - 1;
-            const float c = lane_of(v, from);
-            if (c > last) {
-                list_insert(s, c, __builtin_amdgcn_readlane(id, from), lane);
-                last = lane_of(s.list, a.n_top - 1);
+    if (a.n_top) {
+        float over = below_nth(best, a.n_top, -INFINITY);
+        __shared__ int which[kMaxParts];  // the parts that have anything above it
+        const unsigned long long first = __builtin_amdgcn_ballot_w64(best[0] > over), second = __builtin_amdgcn_ballot_w64(best[1] > over), below = (1ull << lane) - 1;
+        const int n_first = __builtin_popcountll(first), n = (n_first + __builtin_popcountll(second)) * a.n_top;
+        if (best[0] > over) which[__builtin_popcountll(first & below)] = lane;
+        if (best[1] > over) which[n_first + __builtin_popcountll(second & below)] = lane + 64;
+        __syncthreads();
+        constexpr int kAhead = 8;
+        for (int i0 = 0; i0 < n; i0 += 64 * kAhead) {
+            float v[kAhead];
+            int id[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int i = i0 + 64 * k + lane, nth = min(i, n - 1) / a.n_top;
+                const float *at = rows + which[nth] * width + 5 + min(i, n - 1) - nth * a.n_top;
+                v[k] = i < n ? at[0] : -INFINITY;
+                id[k] = __builtin_bit_cast(int, at[a.n_top]);
+            }
+            over = below_nth(v, a.n_top, over);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                unsigned long long in = __builtin_amdgcn_ballot_w64(v[k] > over);
+                while (in) {
+                    const int from = __builtin_ctzll(in);
+                    in &= in - 1;
+                    list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[k]), from)), __builtin_amdgcn_readlane(id[k], from));
+                }
             }
         }
     }
-    const int target = a.target[row];
-    const bool in_range = target >= 0 && target < a.vocab;
-    const float given = in_range ? load_value<T>(static_cast<const Bits *>(a.logits) + row * a.stride + target) : 0.0f;
     write_row<T>(a, row, s, given, in_range, lane);
 }
 
-// Parts per row: enough waves for the chip, one batch a part at least.
+// Parts per row: 4096 waves for the chip (2048 x 128256 bf16, 20 best: one part a row 134 us, two 127, three 139: every part fills a list of its own), a batch a
+// part at least.  Up to four go into one workgroup, as 1, 2 or 4.
 static int score_parts(int64_t n_rows, int64_t vocab) {
-    const int64_t batches = (vocab + kBatch - 1) / kBatch;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(4096 + n_rows - 1) / n_rows, batches, kMaxParts})));
+    const int64_t batches = (vocab + 1023) / 1024;
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(env_int("CAMELID_HIP_SCORE_WAVES", 4096) + n_rows - 1) / n_rows, batches, kMaxParts})));
+    return parts == 3 ? 4 : parts;
 }
 
 size_t token_log_probs_workspace(int64_t n_rows, int64_t vocab, int n_top) {
     const int parts = score_parts(n_rows, vocab);
-    return parts == 1 ? 0 : static_cast<size_t>(n_rows) * parts * partial_floats(n_top) * sizeof(float);
+    return parts <= 4 ? 0 : static_cast<size_t>(n_rows) * parts * partial_floats(n_top) * sizeof(float);
 }
 
 int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_t n_rows, int64_t vocab, const int32_t *target, int n_top, float *log_prob, int32_t *rank, float *entropy,
@@ -248,10 +373,13 @@ int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_
     const ScoreArgs a{logits, target, log_prob, entropy, top_log_probs, rank, top_ids, static_cast<float *>(workspace), stride, n_rows, static_cast<int>(vocab), n_top, score_parts(n_rows, vocab)};
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        CML_COUNT_LAUNCH("score.rows");
-        hipLaunchKernelGGL(token_log_probs_kernel<T>, dim3(static_cast<unsigned>((n_rows * a.parts + 3) / 4)), dim3(256), 0, st, a);
-        if (a.parts > 1) {
-            CML_COUNT_LAUNCH("score.join");
+        const dim3 grid(static_cast<unsigned>((n_rows * a.parts + 3) / 4));
+        if (a.parts <= 4) {
+            CML_COUNT_LAUNCH("score.rows");
+            hipLaunchKernelGGL((token_log_probs_kernel<T, true>), grid, dim3(256), 0, st, a);
+        } else {
+            CML_COUNT_LAUNCH("score.parts");
+            hipLaunchKernelGGL((token_log_probs_kernel<T, false>), grid, dim3(256), 0, st, a);
             hipLaunchKernelGGL(token_log_probs_join_kernel<T>, dim3(static_cast<unsigned>(n_rows)), dim3(64), 0, st, a);
         }
         CML_HIP_TRY(hipGetLastError());

@@ -68,6 +68,17 @@ def test_sizes(t, n, vocab, top, pad, offset):
     compare(t, to_bits(v, t), rng.integers(vocab, size=n), top, pad=pad, offset=offset)
 
 
+# parts as long as they can be, a row of one part, and a part a batch
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("waves,vocab", [(1, 60000), (1, 65536), (1, 65537), (1, 200000), (9, 131072), (4096, 30000)])
+def test_rows_cut_otherwise(t, waves, vocab):
+    rng = np.random.default_rng(vocab)
+    v = (2 * rng.standard_normal((3, vocab))).astype(np.float32)
+    v[1] = np.sort(v[1])
+    with G.env(CAMELID_HIP_SCORE_WAVES=waves):
+        compare(t, to_bits(v, t), np.array([vocab - 1, vocab // 2, 65535 % vocab]), 20)
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 @pytest.mark.parametrize("kind", ["alike", "ascending", "descending", "few_values", "one_high_last", "grid"])
 def test_orders_and_ties(t, kind):
@@ -167,7 +178,7 @@ def test_refusals():
     for kw in (dict(dtype=1 << 8), dict(x=None), dict(t=None), dict(p=None), dict(i=None), dict(a=None), dict(ws=None), dict(x=x.ptr + 2), dict(ws=ws.ptr + 4), dict(h=h.ptr + 1)):
         assert status(**kw) == 2, kw
         assert L.cml_last_error()
-    for kw in (dict(n=-1), dict(v=0), dict(v=(1 << 30) + 1), dict(top=-1), dict(top=65), dict(st=vocab - 1), dict(nb=need - 1)):
+    for kw in (dict(n=-1), dict(v=0), dict(v=(1 << 30) + 1, st=(1 << 30) + 1), dict(top=-1), dict(top=65), dict(st=vocab - 1), dict(nb=need - 1)):
         assert status(**kw) == 3, kw
     assert L.cml_token_log_probs_workspace_bytes(-1, 5, 1) == 0
     check(L.cml_stream_sync(None))
