@@ -37,51 +37,6 @@ __device__ __forceinline__ void store_cells(const MatmulI8 &a, int t, int r, con
         }
 }
 
-// Any alignment and size: 64 rows x 64 tokens a workgroup of four waves, 64 values of the contraction a step, staged through registers.
-template <class T>
-__global__ __launch_bounds__(256) void matmul_i8_kernel(MatmulI8 a) {
-    constexpr int kPitch = 80;  // bytes
-    __shared__ __align__(16) int8_t sw[64 * kPitch], sq[64 * kPitch];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r0 = blockIdx.x * 64, t0 = blockIdx.y * 64;
-    const int row = tid >> 2, k_at = (tid & 3) * 16;
-    const int8_t *w = a.w + min(r0 + row, a.rows - 1) * a.w_stride, *q = a.q + min(t0 + row, a.n_tokens - 1) * a.q_stride;
-    auto piece = [&](const int8_t *p, int k) {
-        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(1)));
-        if (k + 16 <= a.cols) {
-            const v4u v = *reinterpret_cast<const v4u *>(p + k);
-            return make_uint4(v.x, v.y, v.z, v.w);
-        }
-        uint32_t v[4] = {0, 0, 0, 0};
-        for (int j = 0; j < 16; j++)
-            if (k + j < a.cols) v[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[k + j])) << (8 * (j & 3));
-        return make_uint4(v[0], v[1], v[2], v[3]);
-    };
-    v4i_i8 acc[2][2] = {};
-    const int wr = (wave & 1) * 32, wt = (wave >> 1) * 32, n = lane & 15, kq = (lane >> 4) * 16;
-    for (int k = 0; k < a.cols; k += 64) {
-        const uint4 pw = piece(w, k + k_at), pq = piece(q, k + k_at);
-        __syncthreads();
-        *reinterpret_cast<uint4 *>(sw + row * kPitch + k_at) = pw;
-        *reinterpret_cast<uint4 *>(sq + row * kPitch + k_at) = pq;
-        __syncthreads();
-        v4i_i8 fw[2], fq[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            fw[i] = *reinterpret_cast<const v4i_i8 *>(sw + (wr + 16 * i + n) * kPitch + kq);
-            fq[i] = *reinterpret_cast<const v4i_i8 *>(sq + (wt + 16 * i + n) * kPitch + kq);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) store_cells<T>(a, t0 + wt + 16 * j + n, r0 + wr + 16 * i + 4 * (lane >> 4), acc[i][j]);
-}
-
 // ---- few tokens -----------------------------------------------------------------------------------------
 // Up to 16 tokens: the weight's bytes are the time.  A workgroup owns 16 weight rows; its waves take the 128-byte lines of the rows in turn, so that all
 // of a short row is requested at once, and their sums meet in LDS.  Operands go from memory to registers: lane 16 k + n holds 16 bytes of row
@@ -198,7 +153,7 @@ struct TileWork {
     static constexpr int kWaves = WR * WT, kThreads = 64 * kWaves, kRows = WR * MT * 32, kTokens = WT * NT * 32;
     static constexpr int kPass = kThreads / 8;  // rows that one pass of the workgroup fetches
     static constexpr int kStage = (kRows + kTokens) * KB, kFetches = (kRows + kTokens) / kPass, kWeightFetches = kRows / kPass;
-    static constexpr int kTouch = STAGES == 2, kParts = KB / 32;
+    static constexpr int kTouch = FULL, kParts = KB / 32;
     static constexpr int kScales = STAGES * kStage + kTouch * kWaves * 256, kLds = kScales + 8 * kRows;  // stages, what touch() fills, scales and bias of the rows
     static_assert((kRows + kTokens) % kPass == 0 && kRows % kPass == 0, "whole passes of the workgroup");
 
@@ -356,15 +311,18 @@ struct TileWork {
             }
         __builtin_amdgcn_sched_barrier(0);
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = v16i_i8{};
+    }
     // The sums of the tile that aim() and start() began.
     template <int SPLIT>
     __device__ __forceinline__ void sums(uint4 *smem) {
         constexpr int kN = fetches<SPLIT>();
         const int8_t *w0 = weights(), *q0 = tokens();
-#pragma unroll
-        for (int i = 0; i < MT / SPLIT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) acc[i][j] = v16i_i8{};
+        clear();
         if (n_steps > 0) {
             wide_wait<(STAGES - 2) * kN + kTouch>();
             wide_barrier();
@@ -497,6 +455,75 @@ __global__ __launch_bounds__(64 * WR * WT, WR * WT * PER_CU / 4) void matmul_i8_
     work.template store<1>(smem, row, token);
 }
 
+// Rows that start anywhere: a workgroup a tile, through registers (which takes any address), two steps ahead, zeros behind the rows' ends.
+template <class T, int MT>
+__global__ __launch_bounds__(256) void matmul_i8_staged_kernel(MatmulI8 a, TileGrid grid) {
+    extern __shared__ uint4 smem[];
+    typedef TileWork<T, 2, 2, MT, MT, 2, false, false> Work;
+    Work work(a, smem);
+    constexpr int kFetches = Work::kFetches;
+    const int total = grid.n_row_blocks * grid.n_token_blocks, per = total >> 3, more = total & 7, xcd = blockIdx.x & 7;
+    int row_block, token_block, wide;
+    tile_of(grid, xcd * per + min(xcd, more) + (blockIdx.x >> 3), row_block, token_block, wide);
+    const int row = row_block * Work::kRows, token = token_block * Work::kTokens, n_steps = (a.cols + 127) >> 7;
+    const int tid = threadIdx.x, slot = tid & 7;
+    const int8_t *from[kFetches];
+    int piece[kFetches];
+#pragma unroll
+    for (int k = 0; k < kFetches; k++) {
+        const int at = k * Work::kPass + (tid >> 3), t = at - Work::kRows;
+        piece[k] = 16 * (k < Work::kWeightFetches ? slot ^ Work::key_w(at) : slot ^ Work::key_q(t));
+        from[k] = (k < Work::kWeightFetches ? a.w + min(row + at, a.rows - 1) * a.w_stride : a.q + min(token + t, a.n_tokens - 1) * a.q_stride) + piece[k];
+    }
+    auto request = [&](int step, uint4 (&v)[kFetches]) __attribute__((always_inline)) {
+        typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(1)));
+        if ((step + 1) * 128 <= a.cols) {
+#pragma unroll
+            for (int k = 0; k < kFetches; k++) {
+                const v4u w = *reinterpret_cast<const v4u *>(from[k] + step * 128);
+                v[k] = make_uint4(w.x, w.y, w.z, w.w);
+            }
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < kFetches; k++) {
+            const int8_t *p = from[k] + step * 128;
+            const int c = step * 128 + piece[k];
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (c + 16 <= a.cols) {
+                const v4u w = *reinterpret_cast<const v4u *>(p);
+                v[k] = make_uint4(w.x, w.y, w.z, w.w);
+            } else if (c < a.cols) {
+                uint32_t b[4] = {0, 0, 0, 0};
+                for (int j = 0; c + j < a.cols; j++) b[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * (j & 3));
+                v[k] = make_uint4(b[0], b[1], b[2], b[3]);
+            }
+        }
+    };
+    uint4 even[kFetches], odd[kFetches];
+    work.clear();
+    auto step = [&](int s, uint4 (&v)[kFetches]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < kFetches; k++) smem[((s & 1) * Work::kStage + k * 16 * Work::kThreads) / 16 + tid] = v[k];
+        if (s + 2 < n_steps) request(s + 2, v);
+        wide_barrier();  // (one a step: the other stage is not written again before every wave is through this step's)
+        work.template read<1>(s & 1, 0);
+#pragma unroll
+        for (int part = 0; part < Work::kParts; part++) {
+            if (part + 1 < Work::kParts) work.template read<1>(s & 1, part + 1);
+            work.template multiply<1, false>(nullptr, nullptr, part, 0, 0);
+        }
+    };
+    request(0, even);
+    if (n_steps > 1) request(1, odd);
+    for (int s = 0; s < n_steps; s += 2) {
+        step(s, even);
+        if (s + 1 < n_steps) step(s + 1, odd);
+    }
+    wide_barrier();
+    work.template store<1>(smem, row, token);
+}
+
 // A workgroup a compute unit, 32 an XCD: each walks the tiles of its XCD's run 32 apart, and asks for the next tile's first step before it stores the one
 // it has.  The tiles that are left when all 32 can no longer have a whole one are cut into halves or quarters of their rows where that gives every
 // unit some (896 tiles, 4096 tokens on 14336 rows: the time of 3.5 tiles instead of 4).  The last tiles of a side that is no whole number of them reach back
@@ -571,6 +598,18 @@ static int launch_tile(const MatmulI8 &a, hipStream_t st) {
     typedef TileWork<T, WR, WT, MT, NT, STAGES, ONCE, false> Work;
     static_assert(Work::kLds * PER_CU <= 160 * 1024, "LDS");
     const auto kernel = matmul_i8_tile_kernel<T, WR, WT, MT, NT, STAGES, PER_CU, ONCE>;
+    static std::atomic<bool> raised{false};
+    if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
+    const TileGrid grid = tile_grid(a, Work::kRows, Work::kTokens);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid.n_row_blocks * grid.n_token_blocks)), dim3(Work::kThreads), Work::kLds, st, a, grid);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+
+template <class T, int MT>
+static int launch_staged(const MatmulI8 &a, hipStream_t st) {
+    typedef TileWork<T, 2, 2, MT, MT, 2, false, false> Work;
+    const auto kernel = matmul_i8_staged_kernel<T, MT>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
     const TileGrid grid = tile_grid(a, Work::kRows, Work::kTokens);
@@ -667,12 +706,9 @@ int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int
         return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
     }
     CML_COUNT_LAUNCH("i8.matmul.staged");
-    return with_type(dtype, [&](auto t) {
-        const dim3 grid(static_cast<unsigned>((rows + 63) / 64), static_cast<unsigned>((n_tokens + 63) / 64));
-        hipLaunchKernelGGL(matmul_i8_kernel<decltype(t)>, grid, dim3(256), 0, st, a);
-        CML_HIP_TRY(hipGetLastError());
-        return CML_OK;
-    });
+    // 128 x 128 where that still is a workgroup for every compute unit
+    const bool large = (rows + 127) / 128 * ((n_tokens + 127) / 128) >= 256;
+    return with_type(dtype, [&](auto t) { return large ? launch_staged<decltype(t), 2>(a, st) : launch_staged<decltype(t), 1>(a, st); });
 }
 
 }  // namespace cml
