@@ -730,7 +730,7 @@ static int bad_f32(const char *what, const void *p) {
     if (reinterpret_cast<uintptr_t>(p) & 3u) return fail(CML_ERR_INVALID, "%s is not 4-byte aligned", what);
     return CML_OK;
 }
-constexpr int64_t kMostI8Row = 65536;      // values of a row that the quantizing kernels hold in registers
+constexpr int64_t kMostI8Row = 1 << 24;    // values of a row that one workgroup quantizes
 constexpr int64_t kMostI8Cols = 131071;    // |sum| <= 2^14 * cols stays below 2^31
 constexpr int64_t kMostRows = 1 << 30;     // rows or tokens of one call: a grid's workgroups are counted in 31 bits
 

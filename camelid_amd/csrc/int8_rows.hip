@@ -26,9 +26,27 @@ struct NormRows {
     float eps;
 };
 
+// What a row's sum of squares and largest |h * weight| (as bits) make of it.
+struct RowScale {
+    float inv, scale, lift, to_q;
+    bool live;
+    __device__ __forceinline__ int quant(float hw) const { return live ? static_cast<int>(fminf(fmaxf(rintf(hw * lift * to_q), -127.0f), 127.0f)) : 0; }
+};
+template <bool NORM>
+__device__ __forceinline__ RowScale row_scale(const NormRows &a, float sum, uint32_t top) {
+    RowScale f;
+    const float most = __builtin_bit_cast(float, top);
+    f.inv = NORM ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : 1.0f;
+    f.scale = most * f.inv / 127.0f;
+    f.lift = most < 1e-30f ? 18446744073709551616.0f : 1.0f;  // 127 / most of a row of tiny values would be infinite: such a row is lifted by 2^64 first
+    f.live = most > 0.0f && fabsf(f.scale) < INFINITY;       // an empty row, or one with an infinity or a NaN in it (its scale is NaN or infinite): no quants
+    f.to_q = f.live ? 127.0f / (most * f.lift) : 0.0f;
+    return f;
+}
+
 // A row by THREADS threads that hold CH times eight values each; workgroups of 256 threads at least, so rows of one wave go four to a workgroup.
-// NORM: the norm above; otherwise y = x.
-template <class T, bool NORM, int THREADS, int CH>
+// NORM: the norm above; otherwise y = x.  ONCE: x and residual are read past the caches.
+template <class T, bool NORM, int THREADS, int CH, bool ONCE>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rows_to_i8_kernel(NormRows a) {
     typedef typename T::Bits Bits;
     constexpr int kWaves = THREADS / 64, kRows = THREADS < 256 ? 256 / THREADS : 1;
@@ -42,32 +60,46 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rows_to_i8_kern
     float h[CH][8], hw[CH][8];
     float sum = 0.0f;
     uint32_t top = 0;  // |h * weight| as bits: they order like the values, and a NaN is above all
+    auto weigh = [&](int c, float (&out)[8]) __attribute__((always_inline)) {
+        const int i = (c * THREADS + tid) * 8;
+        if (!NORM) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) out[j] = h[c][j];
+        } else {
+            if (i + 8 <= a.cols) {
+                load8<TypeF32>(a.weight + i, out);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) out[j] = i + j < a.cols ? a.weight[i + j] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) out[j] = h[c][j] * out[j];
+        }
+    };
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         const int i = (c * THREADS + tid) * 8;
         if (i + 8 <= a.cols) {
-            load8<T>(x + i, h[c]);
+            load8<T, ONCE>(x + i, h[c]);
             if (NORM && r) {
                 float add[8];
-                load8<T>(r + i, add);
+                load8<T, ONCE>(r + i, add);
 #pragma unroll
                 for (int j = 0; j < 8; j++) h[c][j] = rounded<T>(h[c][j] + add[j]);
             }
-            if (NORM) load8<TypeF32>(a.weight + i, hw[c]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                h[c][j] = hw[c][j] = 0.0f;
+                h[c][j] = 0.0f;
                 if (i + j < a.cols) {
                     h[c][j] = load_value<T>(x + i + j);
                     if (NORM && r) h[c][j] = rounded<T>(h[c][j] + load_value<T>(r + i + j));
-                    if (NORM) hw[c][j] = a.weight[i + j];
                 }
             }
         }
+        weigh(c, hw[c]);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            hw[c][j] = NORM ? h[c][j] * hw[c][j] : h[c][j];
             if (NORM) sum = fmaf(h[c][j], h[c][j], sum);
             top = max(top, __builtin_bit_cast(uint32_t, hw[c][j]) & 0x7fffffffu);
         }
@@ -101,22 +133,16 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rows_to_i8_kern
             top = max(top, s_max[w]);
         }
     }
-    float most = __builtin_bit_cast(float, top);
-    const float inv = NORM ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : 1.0f;
-    const float scale = most * inv / 127.0f;
-    // 127 / most of a row of tiny values would be infinite: such a row is lifted by 2^64 first
-    const float lift = most < 1e-30f ? 18446744073709551616.0f : 1.0f;
-    most = most * lift;
-    const bool live = most > 0.0f && fabsf(scale) < INFINITY;  // an empty row, or one with an infinity or a NaN in it (its scale is NaN or infinite): no quants
-    const float to_q = live ? 127.0f / most : 0.0f;
-    if (tid == 0) a.scales[row] = scale;
+    const RowScale f = row_scale<NORM>(a, sum, top);
+    if (tid == 0) a.scales[row] = f.scale;
     int8_t *q = a.q + row * a.q_stride;
+    float *normed = NORM && a.normed ? a.normed + row * a.cols : nullptr;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
         const int i = (c * THREADS + tid) * 8;
         int v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = live ? static_cast<int>(fminf(fmaxf(rintf(hw[c][j] * lift * to_q), -127.0f), 127.0f)) : 0;
+        for (int j = 0; j < 8; j++) v[j] = f.quant(hw[c][j]);
         if (i + 8 <= a.cols) {
             typedef uint32_t v2u __attribute__((ext_vector_type(2), aligned(1)));
             *reinterpret_cast<v2u *>(q + i) = v2u{pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7])};
@@ -125,43 +151,90 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rows_to_i8_kern
             for (int j = 0; j < 8; j++)
                 if (i + j < a.cols) q[i + j] = static_cast<int8_t>(v[j]);
         }
-    }
-    if (NORM && a.normed) {
-        float *out = a.normed + row * a.cols;
+        if (!normed) continue;
+        float y[8];
 #pragma unroll
-        for (int c = 0; c < CH; c++) {
-            const int i = (c * THREADS + tid) * 8;
-            float y[8];
+        for (int j = 0; j < 8; j++) y[j] = hw[c][j] * f.inv;
+        if (i + 8 <= a.cols) {
+            store8<TypeF32>(normed + i, y);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = hw[c][j] * inv;
-            if (i + 8 <= a.cols) {
-                store8<TypeF32>(out + i, y);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (i + j < a.cols) out[i + j] = y[j];
-            }
+            for (int j = 0; j < 8; j++)
+                if (i + j < a.cols) normed[i + j] = y[j];
         }
+    }
+}
+
+// Rows that the registers do not hold: read twice, the second time from `sum` where it is written (which may be x or residual).
+template <class T, bool NORM>
+__global__ __launch_bounds__(1024) void long_rows_to_i8_kernel(NormRows a) {
+    typedef typename T::Bits Bits;
+    __shared__ float s_sum[16];
+    __shared__ uint32_t s_max[16];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const Bits *x = static_cast<const Bits *>(a.x) + row * a.x_stride;
+    const Bits *r = NORM && a.residual ? static_cast<const Bits *>(a.residual) + row * a.residual_stride : nullptr;
+    Bits *out = NORM && a.sum ? static_cast<Bits *>(a.sum) + row * a.sum_stride : nullptr;
+    auto value = [&](int i) __attribute__((always_inline)) {
+        const float v = load_value<T>(x + i);
+        return r ? rounded<T>(v + load_value<T>(r + i)) : v;
+    };
+    float sum = 0.0f;
+    uint32_t top = 0;
+    for (int i = tid; i < a.cols; i += 1024) {
+        const float h = value(i);
+        if (out) store_value<T>(out + i, h);
+        if (NORM) sum = fmaf(h, h, sum);
+        top = max(top, __builtin_bit_cast(uint32_t, NORM ? h * a.weight[i] : h) & 0x7fffffffu);
+    }
+    sum = wave_allsum(sum);
+    top = static_cast<uint32_t>(wave_allmax_i32(static_cast<int>(top)));
+    if ((tid & 63) == 0) {
+        s_sum[tid >> 6] = sum;
+        s_max[tid >> 6] = top;
+    }
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        sum = sum + s_sum[w];
+        top = max(top, s_max[w]);
+    }
+    const RowScale f = row_scale<NORM>(a, sum, top);
+    if (tid == 0) a.scales[row] = f.scale;
+    for (int i = tid; i < a.cols; i += 1024) {
+        const float h = out ? load_value<T>(out + i) : value(i), hw = NORM ? h * a.weight[i] : h;
+        a.q[row * a.q_stride + i] = static_cast<int8_t>(f.quant(hw));
+        if (NORM && a.normed) a.normed[row * a.cols + i] = hw * f.inv;
     }
 }
 
 template <class T, bool NORM, int THREADS, int CH>
 static int launch_rows(const NormRows &a, hipStream_t st) {
     constexpr int kThreads = THREADS < 256 ? 256 : THREADS, kRows = kThreads / THREADS;
-    hipLaunchKernelGGL((rows_to_i8_kernel<T, NORM, THREADS, CH>), dim3(static_cast<unsigned>((a.n_rows + kRows - 1) / kRows)), dim3(kThreads), 0, st, a);
+    const dim3 grid(static_cast<unsigned>((a.n_rows + kRows - 1) / kRows));
+    // Rows of 16-bit values that no cache holds go past them, and leave them to the quants, which are read next (us with cml_dequantize_i8 behind it, plain / so: 8192 x 4096
+    // bf16 64.6 / 63.2, 4096 x 8192 67.6 / 60.1, 8192 x 8192 128.6 / 115.1; 512 x 4096 8.9 / 10.0; f32 4096 x 4096 51.5 / 53.9).
+    if (sizeof(typename T::Bits) == 2 && a.n_rows * a.cols >= 16ll << 20) hipLaunchKernelGGL((rows_to_i8_kernel<T, NORM, THREADS, CH, true>), grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((rows_to_i8_kernel<T, NORM, THREADS, CH, false>), grid, dim3(kThreads), 0, st, a);
     CML_HIP_TRY(hipGetLastError());
     return CML_OK;
 }
 
 template <class T, bool NORM>
 static int launch_rows_typed(const NormRows &a, hipStream_t st) {
+    // Most threads that still have 16 bytes of a 16-bit row each, up to 8192 values (us with cml_dequantize_i8 behind it, 256 / 512 / 1024 threads: 1 x 4096 4.8 / 4.2 / 4.9, 512 x 8192
+    // 16.0 / 13.9 / 14.3, 8192 x 4096 61.6 / 63.2 / 85.9, 8192 x 8192 120 / 115 / 118); 1 x 16384 with 512 / 1024 7.1 / 6.7, 2048 x 16384 66.3 / 63.1.
     if (a.cols <= 512) return launch_rows<T, NORM, 64, 1>(a, st);
     if (a.cols <= 2048) return launch_rows<T, NORM, 256, 1>(a, st);
-    if (a.cols <= 4096) return launch_rows<T, NORM, 256, 2>(a, st);
-    if (a.cols <= 8192) return launch_rows<T, NORM, 256, 4>(a, st);
+    if (a.cols <= 4096) return launch_rows<T, NORM, 512, 1>(a, st);
+    if (a.cols <= 8192) return launch_rows<T, NORM, 512, 2>(a, st);
     if (a.cols <= 16384) return launch_rows<T, NORM, 1024, 2>(a, st);
     if (a.cols <= 32768) return launch_rows<T, NORM, 1024, 4>(a, st);
-    return launch_rows<T, NORM, 1024, 8>(a, st);
+    hipLaunchKernelGGL((long_rows_to_i8_kernel<T, NORM>), dim3(static_cast<unsigned>(a.n_rows)), dim3(1024), 0, st, a);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
 }
 
 int launch_add_rms_norm_i8(int dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const float *weight, float eps, int64_t n_tokens, int64_t cols,

@@ -54,11 +54,13 @@ __device__ __forceinline__ float rounded(float v) {
 
 // Eight neighbouring values.  The address only has to be aligned to the element: global loads and stores of 16 bytes take any
 // address on this chip (rows of an odd number of values start anywhere).
-template <class T>
+// ONCE: with the non-temporal hint.
+template <class T, bool ONCE = false>
 __device__ __forceinline__ void load8(const typename T::Bits *p, float (&v)[8]) {
     if constexpr (sizeof(typename T::Bits) == 4) {
         typedef float v4f __attribute__((ext_vector_type(4), aligned(4)));
-        const v4f a = reinterpret_cast<const v4f *>(p)[0], b = reinterpret_cast<const v4f *>(p)[1];
+        const v4f *q = reinterpret_cast<const v4f *>(p);
+        const v4f a = ONCE ? __builtin_nontemporal_load(q) : q[0], b = ONCE ? __builtin_nontemporal_load(q + 1) : q[1];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             v[i] = a[i];
@@ -66,7 +68,8 @@ __device__ __forceinline__ void load8(const typename T::Bits *p, float (&v)[8]) 
         }
     } else {
         typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
-        const v4u a = *reinterpret_cast<const v4u *>(p);
+        const v4u *q = reinterpret_cast<const v4u *>(p);
+        const v4u a = ONCE ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             v[2 * i] = T::widen(a[i] & 0xffffu);

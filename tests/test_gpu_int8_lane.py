@@ -59,7 +59,7 @@ def check_norm(t, x, residual, weight, eps, got):
 # one value; odd; the last of one wave; either side of every number of values a thread holds; the longest
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,cols,pad,offset", [(1, 1, 0, 0), (5, 7, 3, 1), (9, 512, 0, 0), (3, 513, 0, 0), (4, 2048, 8, 8), (2, 2049, 1, 3), (3, 4096, 0, 0), (2, 4100, 0, 0),
-                                               (2, 8193, 0, 1), (1, 16384, 0, 0), (1, 16391, 0, 0), (1, 40000, 0, 0), (1, 65536, 0, 0), (2100, 96, 0, 0)])
+                                               (2, 8193, 0, 1), (1, 16384, 0, 0), (1, 16391, 0, 0), (1, 40000, 0, 0), (1, 65536, 0, 0), (2, 32768, 0, 0), (3, 32770, 3, 0), (2100, 96, 0, 0)])
 def test_norm_sizes(t, n, cols, pad, offset):
     rng = np.random.default_rng(cols + n)
     channel = np.exp(0.5 * rng.standard_normal(cols))
@@ -69,10 +69,11 @@ def test_norm_sizes(t, n, cols, pad, offset):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
-def test_norm_without_residual_in_place_and_without_the_optional_outputs(t):
+@pytest.mark.parametrize("cols", [1000, 40001])
+def test_norm_without_residual_in_place_and_without_the_optional_outputs(t, cols):
     rng = np.random.default_rng(3)
-    x, r = to_bits(rng.standard_normal((6, 1000)), t), to_bits(rng.standard_normal((6, 1000)), t)
-    w = (0.5 + rng.random(1000)).astype(np.float32)
+    x, r = to_bits(rng.standard_normal((6, cols)), t), to_bits(rng.standard_normal((6, cols)), t)
+    w = (0.5 + rng.random(cols)).astype(np.float32)
     w[5] = -2.0
     full = norm(t, x, r, w, 1e-6)
     check_norm(t, x, None, w, 1e-6, norm(t, x, None, w, 1e-6))
@@ -227,12 +228,12 @@ def test_refusals():
         assert L.cml_last_error()
     for kw in (dict(n=-1), dict(cols=-1), dict(xs=63), dict(qs=63), dict(r=x.ptr, rs=8), dict(s=o.ptr, ss=63), dict(n=(1 << 30) + 1)):
         assert norm_status(**kw) == 3, kw
-    assert norm_status(cols=65537, xs=65537, qs=65537, n=1) == 6
+    assert norm_status(cols=(1 << 24) + 1, xs=(1 << 24) + 1, qs=(1 << 24) + 1, n=1) == 6
 
     assert L.cml_quantize_i8(0, x.ptr, 64, 4, 64, q.ptr, 64, d.ptr, None) == 0
     assert L.cml_quantize_i8(7, x.ptr, 64, 4, 64, q.ptr, 64, d.ptr, None) == 2
     assert L.cml_quantize_i8(0, x.ptr, 63, 4, 64, q.ptr, 64, d.ptr, None) == 3
-    assert L.cml_quantize_i8(0, x.ptr, 1 << 20, 1, 1 << 20, q.ptr, 1 << 20, d.ptr, None) == 6
+    assert L.cml_quantize_i8(0, x.ptr, 1 << 25, 1, 1 << 25, q.ptr, 1 << 25, d.ptr, None) == 6
     assert L.cml_dequantize_i8(q.ptr, 64, d.ptr, 4, 64, 0, o.ptr, 64, None) == 0
     assert L.cml_dequantize_i8(q.ptr, 64, None, 4, 64, 0, o.ptr, 64, None) == 2
     assert L.cml_dequantize_i8(q.ptr, 64, d.ptr, 4, 64, 3, o.ptr, 64, None) == 2
