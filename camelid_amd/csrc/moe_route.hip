@@ -10,7 +10,8 @@
 // An expert whose logit is NaN or -inf, or whose key is, takes no part; a token left with fewer than k experts has id -1 and weight 0 in the slots behind
 // them (the expert lane drops such slots).  +inf counts as the largest finite logit.
 //
-// One wave per token, lane l holding the NE neighbouring experts from l * NE: the lowest lane of a ballot is the lowest index.
+// A token has a whole wave, or 16 lanes of one.  A group has 1, 2, 4, 8 or 16 lanes and each of them `per` neighbouring experts (the group's last one maybe
+// fewer): what is ahead in lane and place has the lower index.
 #include <type_traits>
 
 #include "typed_rows.hpp"
@@ -27,135 +28,148 @@ struct RouteArgs {
     int64_t stride, n_tokens;
     int n_experts, n_groups, groups_kept, group_top, k;
     int group_size;
-    int group_lanes;        // lanes that hold a group, or 0: no power of two up to 16
-    uint32_t size_inverse;  // ceil(2^20 / group_size): e / group_size = e * size_inverse >> 20 for e < 1024
+    int group_shift;  // log2 of the lanes that hold a group
+    int per;          // experts per lane
     int renormalise;
     float weight_scale;
 };
 
 constexpr int kOut = INT32_MIN;  // key of an expert that takes no part: below every ordered float
 
-template <class T, bool SIGMOID, int NE>
-__global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
-    typedef typename T::Bits Bits;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-    if (t >= a.n_tokens) return;  // (a wave's work is its own: no barriers)
-    const Bits *lg = static_cast<const Bits *>(a.logits) + t * a.stride;
-    float score[NE];
-    int key[NE];
-    bool in[NE];
+// The experts of a lane.
+struct LaneExperts {
+    int first, count;
+    __device__ __forceinline__ LaneExperts(const RouteArgs &a, int lane) {
+        const int group = lane >> a.group_shift, at = (lane & ((1 << a.group_shift) - 1)) * a.per;
+        first = group * a.group_size + at;
+        count = group < a.n_groups ? max(0, min(a.per, a.group_size - at)) : 0;
+    }
+};
+
+// Their values, -inf behind the last.
+template <class T, int NE>
+__device__ __forceinline__ void load_experts(const typename T::Bits *p, const LaneExperts &my, float (&v)[NE]) {
+    if constexpr (NE >= 8) {
+        if (my.count == NE) {
+#pragma unroll
+            for (int j = 0; j < NE; j += 8) {
+                float eight[8];
+                load8<T>(p + my.first + j, eight);
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[j + i] = eight[i];
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NE; j++) v[j] = -INFINITY;
+    if (my.count > 0)
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            const float here = load_value<T>(p + my.first + min(j, my.count - 1));
+            v[j] = j < my.count ? here : -INFINITY;
+        }
+}
+
+// Scores and values (the floats behind the keys) of a lane's experts; LANES lanes have the token.  in: takes part; the value of one that does not is -inf.
+template <class T, bool SIGMOID, int NE, int LANES>
+__device__ __forceinline__ void rate_experts(const RouteArgs &a, int64_t t, const LaneExperts &my, float (&score)[NE], float (&value)[NE], bool (&in)[NE]) {
     float most = -3.4028235e38f;
+    load_experts<T, NE>(static_cast<const typename T::Bits *>(a.logits) + t * a.stride, my, value);
 #pragma unroll
     for (int j = 0; j < NE; j++) {
-        const int e = lane * NE + j;
-        float v = e < a.n_experts ? load_value<T>(lg + e) : -INFINITY;
-        in[j] = v > -INFINITY;  // (false for NaN)
-        v = fminf(v, 3.4028235e38f);
-        score[j] = v;
-        if (in[j]) most = fmaxf(most, v);
+        in[j] = value[j] > -INFINITY;  // (false for NaN)
+        value[j] = fminf(value[j], 3.4028235e38f);
+        if (in[j]) most = fmaxf(most, value[j]);
     }
-    float total = 1.0f;
-    if constexpr (!SIGMOID) most = from_total_key(wave_allmax_i32(total_key(most)));
-    float logit[NE];
+    if constexpr (SIGMOID) {
 #pragma unroll
-    for (int j = 0; j < NE; j++) {
-        logit[j] = score[j];
-        if constexpr (SIGMOID) score[j] = in[j] ? 1.0f / (1.0f + expf(-logit[j])) : 0.0f;
-        else score[j] = in[j] ? expf(logit[j] - most) : 0.0f;
-    }
-    if constexpr (!SIGMOID) {
+        for (int j = 0; j < NE; j++) score[j] = in[j] ? 1.0f / (1.0f + expf(-value[j])) : 0.0f;
+    } else {
+        most = from_total_key(LANES == 64 ? wave_allmax_i32(total_key(most)) : row_allmax_i32(total_key(most)));
         float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NE; j++) sum = sum + score[j];
-        total = wave_allsum(sum);
+        for (int j = 0; j < NE; j++) {
+            score[j] = in[j] ? expf(value[j] - most) : 0.0f;
+            sum = sum + score[j];
+        }
+        const float total = LANES == 64 ? wave_allsum(sum) : row_allsum(sum);
         if (total > 0.0f)
 #pragma unroll
             for (int j = 0; j < NE; j++) score[j] = score[j] / total;
     }
-    float value[NE];
+    if (a.bias) {
+        float bias[NE];
+        load_experts<TypeF32, NE>(a.bias, my, bias);
+#pragma unroll
+        for (int j = 0; j < NE; j++) value[j] = score[j] + bias[j];
+    }
 #pragma unroll
     for (int j = 0; j < NE; j++) {
-        const int e = lane * NE + j;
-        value[j] = a.bias && in[j] ? score[j] + a.bias[e] : logit[j];
         in[j] = in[j] && value[j] > -INFINITY;
-        key[j] = in[j] ? total_key(value[j] + 0.0f) : kOut;  // (-0 is 0)
+        value[j] = in[j] ? value[j] + 0.0f : -INFINITY;  // (-0 is 0)
     }
+}
+
+// What a group is rated by: its best keys; without a bias and for two, the scores, which order as the logits do.
+template <int NE>
+__device__ __forceinline__ void group_keys(const RouteArgs &a, const float (&score)[NE], const float (&value)[NE], const bool (&in)[NE], int (&rated)[NE]) {
+#pragma unroll
+    for (int j = 0; j < NE; j++) rated[j] = in[j] ? total_key(a.bias || a.group_top == 1 ? value[j] : score[j]) : kOut;
+}
+__device__ __forceinline__ int group_worth(const RouteArgs &a, int first, int second) {
+    if (first == kOut) return kOut;
+    if (a.group_top == 1 || second == kOut) return first;
+    return total_key(from_total_key(first) + from_total_key(second) + 0.0f);
+}
+// The worth of the group that a lane belongs to: two best per lane, then of pairs of lanes, of fours, ...
+template <int NE>
+__device__ __forceinline__ int lanes_worth(const RouteArgs &a, const int (&rated)[NE]) {
+    int first = kOut, second = kOut;
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        second = max(second, min(first, rated[j]));
+        first = max(first, rated[j]);
+    }
+    auto meet = [&](auto ctrl) __attribute__((always_inline)) {
+        constexpr int kCtrl = decltype(ctrl)::value;
+        const int f = __builtin_amdgcn_update_dpp(0, first, kCtrl, 0xf, 0xf, false), s = __builtin_amdgcn_update_dpp(0, second, kCtrl, 0xf, 0xf, false);
+        second = max(min(first, f), max(second, s));
+        first = max(first, f);
+    };
+    if (a.group_shift >= 1) meet(std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+    if (a.group_shift >= 2) meet(std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+    if (a.group_shift >= 3) meet(std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad
+    if (a.group_shift >= 4) meet(std::integral_constant<int, 0x140>{}); // row_mirror: the other eight
+    return group_worth(a, first, second);
+}
+
+template <class T, bool SIGMOID, int NE>
+__global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+    if (t >= a.n_tokens) return;  // (a wave's work is its own: no barriers)
+    float score[NE], value[NE];
+    bool in[NE];
+    const LaneExperts my(a, lane);
+    rate_experts<T, SIGMOID, NE, 64>(a, t, my, score, value, in);
+    int key[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) key[j] = in[j] ? total_key(value[j]) : kOut;
     if (a.n_groups > 1) {
-        // A group's worth.  Its two best keys: without a bias and for two, of the scores, which order as the logits do.
-        int rated[NE], worth = kOut;
-#pragma unroll
-        for (int j = 0; j < NE; j++) rated[j] = in[j] ? (a.bias || a.group_top == 1 ? key[j] : total_key(score[j])) : kOut;
-        const auto both = [&](int first, int second) __attribute__((always_inline)) {
-            if (first == kOut) return kOut;
-            if (a.group_top == 1 || second == kOut) return first;
-            return total_key(from_total_key(first) + from_total_key(second) + 0.0f);
-        };
-        unsigned long long kept = 0;
-        if (a.group_lanes > 0) {
-            // A group is 1, 2, 4, 8 or 16 whole lanes: two best per lane, then of pairs of lanes, of fours, ...
-            int first = kOut, second = kOut;
-#pragma unroll
-            for (int j = 0; j < NE; j++) {
-                second = max(second, min(first, rated[j]));
-                first = max(first, rated[j]);
-            }
-            auto meet = [&](auto ctrl) __attribute__((always_inline)) {
-                constexpr int kCtrl = decltype(ctrl)::value;
-                const int f = __builtin_amdgcn_update_dpp(0, first, kCtrl, 0xf, 0xf, false), s = __builtin_amdgcn_update_dpp(0, second, kCtrl, 0xf, 0xf, false);
-                second = max(min(first, f), max(second, s));
-                first = max(first, f);
-            };
-            if (a.group_lanes >= 2) meet(std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
-            if (a.group_lanes >= 4) meet(std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
-            if (a.group_lanes >= 8) meet(std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad
-            if (a.group_lanes >= 16) meet(std::integral_constant<int, 0x140>{}); // row_mirror: the other eight
-            worth = both(first, second);
-            // it stays if fewer than groups_kept are ahead of it
-            const int mine = lane / a.group_lanes;
-            int ahead = 0;
-            for (int g = 0; g < a.n_groups; g++) {
-                const int theirs = __builtin_amdgcn_readlane(worth, g * a.group_lanes);
-                ahead += (theirs > worth) | ((theirs == worth) & (g < mine));
-            }
-            if (ahead >= a.groups_kept)
-#pragma unroll
-                for (int j = 0; j < NE; j++) key[j] = kOut;
-        } else {
-            // any size: the groups one after the other, each lane's experts of that group against the wave
-            for (int g = 0; g < a.n_groups; g++) {
-                int best[2] = {kOut, kOut}, taken = -1;
-#pragma unroll 1
-                for (int s = 0; s < a.group_top; s++) {
-                    int most = kOut, at = -1;
-#pragma unroll
-                    for (int j = NE - 1; j >= 0; j--) {
-                        const int e = lane * NE + j;
-                        if (static_cast<int>(e * a.size_inverse >> 20) == g && e != taken && rated[j] >= most) {
-                            most = rated[j];
-                            at = e;
-                        }
-                    }
-                    const int m = wave_allmax_i32(most);
-                    if (m == kOut) break;
-                    taken = __builtin_amdgcn_readlane(at, __builtin_ctzll(__builtin_amdgcn_ballot_w64(most == m)));
-                    best[s] = m;
-                }
-                if (lane == g) worth = both(best[0], best[1]);
-            }
-            for (int s = 0; s < a.groups_kept; s++) {
-                const int m = wave_allmax_i32(worth);
-                if (m == kOut) break;
-                const int g = __builtin_ctzll(__builtin_amdgcn_ballot_w64(worth == m));
-                kept |= 1ull << g;
-                if (lane == g) worth = kOut;
-            }
-#pragma unroll
-            for (int j = 0; j < NE; j++)
-                if (!(kept >> ((lane * NE + j) * a.size_inverse >> 20 & 63) & 1)) key[j] = kOut;
+        int rated[NE];
+        group_keys(a, score, value, in, rated);
+        const int worth = lanes_worth(a, rated), mine = lane >> a.group_shift;
+        int ahead = 0;  // a group stays if fewer than groups_kept are ahead of it
+        for (int g = 0; g < a.n_groups; g++) {
+            const int theirs = __builtin_amdgcn_readlane(worth, g << a.group_shift);
+            ahead += (theirs > worth) | ((theirs == worth) & (g < mine));
         }
+        if (ahead >= a.groups_kept)
+#pragma unroll
+            for (int j = 0; j < NE; j++) key[j] = kOut;
     }
-    int chosen = -1;  // lane s: slot s
+    int place = -1;  // lane s: where slot s is, its lane * NE + j
     for (int s = 0; s < a.k; s++) {
         int best = key[NE - 1], at = NE - 1;
 #pragma unroll
@@ -165,17 +179,19 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
         }
         const int m = wave_allmax_i32(best);
         if (m == kOut) break;
-        const int e = __builtin_amdgcn_readlane(lane * NE + at, __builtin_ctzll(__builtin_amdgcn_ballot_w64(best == m)));
+        const int p = __builtin_amdgcn_readlane(lane * NE + at, __builtin_ctzll(__builtin_amdgcn_ballot_w64(best == m)));
 #pragma unroll
-        for (int j = 0; j < NE; j++) key[j] = e == lane * NE + j ? kOut : key[j];
-        chosen = lane == s ? e : chosen;
+        for (int j = 0; j < NE; j++) key[j] = p == lane * NE + j ? kOut : key[j];
+        place = lane == s ? p : place;
     }
-    // the chosen experts' scores, from the lanes that hold them
+    // the chosen experts and their scores, from the lanes that hold them
+    const int holder = (place < 0 ? 0 : place) / NE;
+    const int chosen = place < 0 ? -1 : LaneExperts(a, holder).first + place % NE;
     float w = 0.0f;
 #pragma unroll
     for (int j = 0; j < NE; j++) {
-        const float theirs = __shfl(score[j], (chosen < 0 ? 0 : chosen) / NE);
-        w = chosen >= 0 && chosen % NE == j ? theirs : w;
+        const float theirs = __shfl(score[j], holder);
+        w = place >= 0 && place % NE == j ? theirs : w;
     }
     if (a.renormalise) {
         const float sum = wave_allsum(w);
@@ -188,28 +204,156 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
     }
 }
 
+// Four tokens a wave, 16 lanes each, for up to 8 of 256 experts.  Every lane sorts its experts first, as doubles: a value's f32 bits are the upper word (finite
+// and infinite floats are finite doubles, in the same order), its place the lower one, so that a comparison that the chip makes at full rate decides ties as well.
+// Then the lanes' first entries meet k times, and the lane that held the best goes on to its next.
+constexpr int kMostSorted = 8;  // chosen at most
+
+__device__ __forceinline__ void sort_two(double &a, double &b) {  // descending
+    const double hi = __builtin_fmax(a, b);
+    b = __builtin_fmin(a, b);
+    a = hi;
+}
+__device__ __forceinline__ void sort_eight(double *v) {  // odd-even merges
+    constexpr int kAt[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6}, {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+    for (int i = 0; i < 19; i++) sort_two(v[kAt[i][0]], v[kAt[i][1]]);
+}
+__device__ __forceinline__ void sort_best(double (&v)[4]) {
+    sort_two(v[0], v[1]);
+    sort_two(v[2], v[3]);
+    sort_two(v[0], v[2]);
+    sort_two(v[1], v[3]);
+    sort_two(v[1], v[2]);
+}
+__device__ __forceinline__ void sort_best(double (&v)[8]) { sort_eight(v); }
+__device__ __forceinline__ void sort_best(double (&v)[16]) {  // the first 8 only
+    sort_eight(v);
+    sort_eight(v + 8);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __builtin_fmax(v[i], v[15 - i]);
+#pragma unroll
+    for (int d = 4; d; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (!(i & d)) sort_two(v[i], v[i + d]);
+}
+
 template <class T, bool SIGMOID, int NE>
-static int launch_route_lanes(RouteArgs a, hipStream_t st) {
-    const int lanes = a.group_size % NE == 0 ? a.group_size / NE : 0;
-    a.group_lanes = lanes <= 16 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+__global__ __launch_bounds__(256) void moe_route_scored_quarter_kernel(RouteArgs a) {
+    constexpr int kEntries = NE < kMostSorted ? NE : kMostSorted;
+    const int token = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + token, here = min(t, a.n_tokens - 1);
+    float score[NE], value[NE];
+    bool in[NE];
+    const LaneExperts my(a, lane);
+    rate_experts<T, SIGMOID, NE, 16>(a, here, my, score, value, in);
+    __shared__ __align__(16) float scores[16][16 * NE];  // (written and read by the same wave)
+#pragma unroll
+    for (int j = 0; j < NE; j++) scores[token][lane * NE + j] = score[j];
+    if (a.n_groups > 1) {
+        int rated[NE];
+        group_keys(a, score, value, in, rated);
+        const int worth = lanes_worth(a, rated), mine = lane >> a.group_shift;
+        int ahead = 0;  // a group stays if fewer than groups_kept are ahead of it
+        for (int g = 0; g < a.n_groups; g++) {
+            const int theirs = __shfl(worth, g << a.group_shift, 16);
+            ahead += (theirs > worth) | ((theirs == worth) & (g < mine));
+        }
+        if (ahead >= a.groups_kept)
+#pragma unroll
+            for (int j = 0; j < NE; j++) value[j] = -INFINITY;
+    }
+    double entry[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        const int bits = __builtin_bit_cast(int, value[j]);
+        entry[j] = __hiloint2double(bits, ~((lane * NE + j) ^ (bits >> 31)));  // (of equal values the one ahead is the larger, of equal negative ones too)
+    }
+    sort_best(entry);
+    int key[kEntries], place[kEntries];
+#pragma unroll
+    for (int i = 0; i < kEntries; i++) {
+        const int bits = __double2hiint(entry[i]);
+        key[i] = total_key(__builtin_bit_cast(float, bits));
+        place[i] = ~__double2loint(entry[i]) ^ (bits >> 31);
+    }
+    const int none = total_key(-INFINITY);
+    int where = -1;  // lane s: slot s
+#pragma unroll
+    for (int s = 0; s < kMostSorted; s++) {
+        if (s == a.k) break;
+        const int m = row_allmax_i32(key[0]);
+        const int p = row_allmin_i32(key[0] == m ? place[0] : INT32_MAX);
+        where = lane == s && m != none ? p : where;
+        const bool next = place[0] == p;
+#pragma unroll
+        for (int i = 0; i < kEntries - 1 && i < kMostSorted - 1 - s; i++) {
+            key[i] = next ? key[i + 1] : key[i];
+            place[i] = next ? place[i + 1] : place[i];
+        }
+        if (s + kEntries < kMostSorted) {
+            key[kEntries - 1] = next ? none : key[kEntries - 1];
+            place[kEntries - 1] = next ? INT32_MAX : place[kEntries - 1];
+        }
+    }
+    const int chosen = where < 0 ? -1 : LaneExperts(a, where / NE).first + where % NE;
+    float w = where >= 0 ? scores[token][where] : 0.0f;
+    if (a.renormalise) {
+        const float sum = row_allsum(w);
+        const int live = __builtin_popcount(static_cast<unsigned>(__builtin_amdgcn_ballot_w64(chosen >= 0) >> (threadIdx.x & 48)) & 0xffffu);
+        w = sum > 0.0f ? w / sum : chosen >= 0 ? 1.0f / static_cast<float>(live) : 0.0f;  // (all chosen scores 0: alike)
+    }
+    if (t < a.n_tokens && lane < a.k) {
+        a.idx[t * a.k + lane] = chosen;
+        a.weight[t * a.k + lane] = w * a.weight_scale;
+    }
+}
+
+template <class T, bool SIGMOID, int NE>
+static int launch_route_wave(const RouteArgs &a, hipStream_t st) {
+    CML_COUNT_LAUNCH("moe.route.scored");
     hipLaunchKernelGGL((moe_route_scored_kernel<T, SIGMOID, NE>), dim3(static_cast<unsigned>((a.n_tokens + 3) / 4)), dim3(256), 0, st, a);
     CML_HIP_TRY(hipGetLastError());
     return CML_OK;
 }
+template <class T, bool SIGMOID, int NE>
+static int launch_route_quarter(const RouteArgs &a, hipStream_t st) {
+    CML_COUNT_LAUNCH("moe.route.scored.quarter");
+    hipLaunchKernelGGL((moe_route_scored_quarter_kernel<T, SIGMOID, NE>), dim3(static_cast<unsigned>((a.n_tokens + 15) / 16)), dim3(256), 0, st, a);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+// The groups over the lanes of a token: a power of two lanes each, 16 at most (what rates them stays inside 16 lanes).
+static bool spread_groups(RouteArgs &a, int lanes, int most_per) {
+    if (a.n_groups > lanes) return false;
+    int shift = 0;
+    while (a.n_groups << (shift + 1) <= lanes && (shift < 4 || a.n_groups == 1)) shift++;
+    a.group_shift = shift;
+    a.per = (a.group_size + (1 << shift) - 1) >> shift;
+    return a.per <= most_per;
+}
 template <class T, bool SIGMOID>
-static int launch_route(const RouteArgs &a, hipStream_t st) {
-    if (a.n_experts <= 64) return launch_route_lanes<T, SIGMOID, 1>(a, st);
-    if (a.n_experts <= 128) return launch_route_lanes<T, SIGMOID, 2>(a, st);
-    if (a.n_experts <= 256) return launch_route_lanes<T, SIGMOID, 4>(a, st);
-    if (a.n_experts <= 512) return launch_route_lanes<T, SIGMOID, 8>(a, st);
-    return launch_route_lanes<T, SIGMOID, 16>(a, st);
+static int launch_route(RouteArgs a, hipStream_t st) {
+    // Four tokens a wave where there are waves enough that way.
+    if (a.n_tokens >= env_int("CAMELID_HIP_ROUTE_QUARTER", 2048) && a.k <= kMostSorted && spread_groups(a, 16, 16)) {
+        if (a.per <= 4) return launch_route_quarter<T, SIGMOID, 4>(a, st);
+        if (a.per <= 8) return launch_route_quarter<T, SIGMOID, 8>(a, st);
+        return launch_route_quarter<T, SIGMOID, 16>(a, st);
+    }
+    spread_groups(a, 64, 32);  // (1024 experts in up to 64 groups come to 32 a lane at most)
+    if (a.per <= 1) return launch_route_wave<T, SIGMOID, 1>(a, st);
+    if (a.per <= 2) return launch_route_wave<T, SIGMOID, 2>(a, st);
+    if (a.per <= 4) return launch_route_wave<T, SIGMOID, 4>(a, st);
+    if (a.per <= 8) return launch_route_wave<T, SIGMOID, 8>(a, st);
+    if (a.per <= 16) return launch_route_wave<T, SIGMOID, 16>(a, st);
+    return launch_route_wave<T, SIGMOID, 32>(a, st);
 }
 
 int launch_moe_route_scored(int score, int dtype, const void *logits, int64_t stride, const float *bias, int64_t n_tokens, int n_experts, int n_groups, int groups_kept, int group_top, int k,
                             int renormalise, float weight_scale, int32_t *idx, float *weight, hipStream_t st) {
     const int size = n_experts / n_groups;
-    const RouteArgs a{logits, bias, idx, weight, stride, n_tokens, n_experts, n_groups, groups_kept, group_top, k, size, 0, ((1u << 20) + size - 1) / size, renormalise, weight_scale};
-    CML_COUNT_LAUNCH("moe.route.scored");
+    const RouteArgs a{logits, bias, idx, weight, stride, n_tokens, n_experts, n_groups, groups_kept, group_top, k, size, 0, 0, renormalise, weight_scale};
     return with_type(dtype, [&](auto t) { return score == CML_ROUTE_SIGMOID ? launch_route<decltype(t), true>(a, st) : launch_route<decltype(t), false>(a, st); });
 }
 

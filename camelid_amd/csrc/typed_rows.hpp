@@ -92,10 +92,28 @@ __device__ __forceinline__ void store8(typename T::Bits *p, const float (&v)[8])
     }
 }
 
-// ---- over the 64 lanes of a wave, the result in every lane; the association is fixed ----------------
+// ---- over the 16 lanes of a row and the 64 of a wave, the same result in every lane; the association is fixed ----
+__device__ __forceinline__ float row_allsum(float v) {
+    v = v + dpp_f32<0xB1>(v);   // quad_perm [1,0,3,2]
+    v = v + dpp_f32<0x4E>(v);   // quad_perm [2,3,0,1]
+    v = v + dpp_f32<0x141>(v);  // row_half_mirror: the other quad
+    return v + dpp_f32<0x140>(v);  // row_mirror: the other eight (both sides add the same two numbers every time)
+}
+__device__ __forceinline__ int row_allmax_i32(int v) {
+    v = max(v, row_ror_i32<1>(v));
+    v = max(v, row_ror_i32<2>(v));
+    v = max(v, row_ror_i32<4>(v));
+    return max(v, row_ror_i32<8>(v));
+}
+__device__ __forceinline__ int row_allmin_i32(int v) {
+    v = min(v, row_ror_i32<1>(v));
+    v = min(v, row_ror_i32<2>(v));
+    v = min(v, row_ror_i32<4>(v));
+    return min(v, row_ror_i32<8>(v));
+}
 __device__ __forceinline__ float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
 __device__ __forceinline__ float wave_allsum(float v) {
-    v = v + dpp_f32<0x121>(v);  // row_ror 1, 2, 4, 8: the sum of the row of 16 in all its lanes
+    v = v + dpp_f32<0x121>(v);  // row_ror 1, 2, 4, 8: the sum of the row of 16 in all its lanes (each with its own association: one lane is read)
     v = v + dpp_f32<0x122>(v);
     v = v + dpp_f32<0x124>(v);
     v = v + dpp_f32<0x128>(v);

@@ -127,6 +127,39 @@ def test_masked_experts_leave_slots_empty(renormalise):
     assert np.array_equal(ids[0], np.arange(5, 13))
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,experts,groups,kept,group_top,k,pad", [(1, 1, 1, 1, 1, 1, 0), (5, 7, 1, 1, 1, 7, 0), (18, 64, 1, 1, 1, 6, 3), (33, 64, 4, 2, 2, 8, 0), (16, 64, 16, 5, 2, 8, 1), (17, 65, 1, 1, 1, 8, 0), (9, 128, 8, 3, 1, 4, 0), (50, 128, 1, 1, 1, 8, 5), (31, 200, 1, 1, 1, 8, 0), (34, 256, 8, 4, 2, 8, 0), (7, 256, 16, 1, 2, 8, 1), (15, 256, 2, 1, 2, 3, 0), (21, 160, 8, 3, 2, 6, 0), (10, 60, 5, 2, 2, 7, 0), (11, 39, 3, 2, 1, 5, 2), (13, 208, 16, 4, 2, 8, 0)])
+def test_four_tokens_a_wave(t, n, experts, groups, kept, group_top, k, pad):
+    """The form that long prompts take, at lengths that leave its last wave part empty."""
+    rng = np.random.default_rng(experts + n)
+    logits = to_bits(rng.integers(-32, 32, (n, experts)) / 8.0, t)
+    bias = (rng.integers(-8, 8, experts) / 64.0).astype(np.float32)
+    with G.env(CAMELID_HIP_ROUTE_QUARTER=1):
+        compare(SIGMOID, t, logits, bias, groups, kept, group_top, k, scale=2.5, pad=pad)
+        compare(SIGMOID, t, logits, -1 - bias, groups, kept, group_top, k, renormalise=0, pad=pad)  # (keys below 0)
+        compare(SOFTMAX, t, logits, None, groups, kept, group_top, k, pad=pad)
+
+
+def test_four_tokens_a_wave_with_masked_experts():
+    with G.env(CAMELID_HIP_ROUTE_QUARTER=1):
+        test_masked_experts_leave_slots_empty(0)
+        test_masked_experts_leave_slots_empty(1)
+
+
+@pytest.mark.parametrize("experts,groups,kept,group_top,k", [(1000, 8, 3, 2, 9), (992, 62, 30, 2, 64), (1023, 33, 5, 2, 8), (1023, 3, 2, 1, 8), (1020, 17, 4, 2, 12), (1024, 2, 1, 2, 8), (39, 13, 4, 1, 5), (77, 7, 3, 2, 3)])
+def test_groups_of_any_size(experts, groups, kept, group_top, k):
+    rng = np.random.default_rng(experts + groups)
+    logits = to_bits(rng.integers(-32, 32, (9, experts)) / 8.0, "f16")
+    compare(SIGMOID, "f16", logits, (rng.integers(-8, 8, experts) / 64.0).astype(np.float32), groups, kept, group_top, k, pad=1)
+
+
+@pytest.mark.parametrize("n", [2047, 2048, 2050])
+def test_long_prompts(n):
+    rng = np.random.default_rng(n)
+    logits = to_bits(rng.integers(-32, 32, (n, 48)) / 8.0, "bf16")
+    compare(SIGMOID, "bf16", logits, (rng.integers(-8, 8, 48) / 64.0).astype(np.float32), 4, 2, 2, 6)
+
+
 def test_results_feed_the_plan():
     """Slots without an expert are dropped by the grouping."""
     v = np.full((3, 16), -np.inf, np.float32)
