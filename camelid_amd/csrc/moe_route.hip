@@ -144,6 +144,8 @@ __device__ __forceinline__ int lanes_worth(const RouteArgs &a, const int (&rated
     return group_worth(a, first, second);
 }
 
+// A wave per token.  The logits are little to read; what it takes is instructions: a sigmoid's exponential and division are 25 for every expert, a turn of the
+// choice about 30, so that 8 of 256 for 8192 tokens (4 MB) come to 11.7 us, where reading them takes 1.  One token: 4.3 us, most of it the launch.
 template <class T, bool SIGMOID, int NE>
 __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -204,44 +206,53 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
     }
 }
 
-// Four tokens a wave, 16 lanes each, for up to 8 of 256 experts.  Every lane sorts its experts first, as doubles: a value's f32 bits are the upper word (finite
+// Four tokens a wave, 16 lanes each, for up to MOST of 16 * NE experts.  Every lane sorts its experts first, as doubles: a value's f32 bits are the upper word (finite
 // and infinite floats are finite doubles, in the same order), its place the lower one, so that a comparison that the chip makes at full rate decides ties as well.
-// Then the lanes' first entries meet k times, and the lane that held the best goes on to its next.
-constexpr int kMostSorted = 8;  // chosen at most
-
+// Then the lanes' first entries meet k times, and the lane that held the best goes on to its next.  A turn's
+// maximum over 16 lanes serves four tokens, so a token takes 250 instructions in place of 600: 8 of 256 for 8192 tokens 8.3 us, two waves to a SIMD and bound by the
+// latency of their chains.
 __device__ __forceinline__ void sort_two(double &a, double &b) {  // descending
     const double hi = __builtin_fmax(a, b);
     b = __builtin_fmin(a, b);
     a = hi;
 }
-__device__ __forceinline__ void sort_eight(double *v) {  // odd-even merges
-    constexpr int kAt[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6}, {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+template <int N>
+__device__ __forceinline__ void sort_bitonic(double *v) {
 #pragma unroll
-    for (int i = 0; i < 19; i++) sort_two(v[kAt[i][0]], v[kAt[i][1]]);
-}
-__device__ __forceinline__ void sort_best(double (&v)[4]) {
-    sort_two(v[0], v[1]);
-    sort_two(v[2], v[3]);
-    sort_two(v[0], v[2]);
-    sort_two(v[1], v[3]);
-    sort_two(v[1], v[2]);
-}
-__device__ __forceinline__ void sort_best(double (&v)[8]) { sort_eight(v); }
-__device__ __forceinline__ void sort_best(double (&v)[16]) {  // the first 8 only
-    sort_eight(v);
-    sort_eight(v + 8);
+    for (int d = N / 2; d; d >>= 1)
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = __builtin_fmax(v[i], v[15 - i]);
-#pragma unroll
-    for (int d = 4; d; d >>= 1)
-#pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < N; i++)
             if (!(i & d)) sort_two(v[i], v[i + d]);
 }
+// The first KEEP of N in order; what is behind them is left in any.
+template <int N, int KEEP>
+__device__ __forceinline__ void sort_best(double *v) {
+    if constexpr (N == 4) {
+        constexpr int kAt[5][2] = {{0, 1}, {2, 3}, {0, 2}, {1, 3}, {1, 2}};
+#pragma unroll
+        for (int i = 0; i < 5; i++) sort_two(v[kAt[i][0]], v[kAt[i][1]]);
+    } else if constexpr (N == 8) {  // odd-even merges
+        constexpr int kAt[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6}, {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+        for (int i = 0; i < 19; i++) sort_two(v[kAt[i][0]], v[kAt[i][1]]);
+    } else {
+        sort_best<N / 2, KEEP>(v);
+        sort_best<N / 2, KEEP>(v + N / 2);
+        constexpr int kHalf = N / 2 < KEEP ? N / 2 : KEEP;  // sorted entries of a half
+#pragma unroll
+        for (int i = 0; i < kHalf; i++) sort_two(v[i], v[N / 2 + kHalf - 1 - i]);
+        if constexpr (kHalf < KEEP) {  // both halves stay: what is behind the larger ones is theirs upside down
+            sort_bitonic<kHalf>(v);
+            sort_bitonic<kHalf>(v + kHalf);
+        } else {
+            sort_bitonic<kHalf>(v);
+        }
+    }
+}
 
-template <class T, bool SIGMOID, int NE>
+template <class T, bool SIGMOID, int NE, int MOST>
 __global__ __launch_bounds__(256) void moe_route_scored_quarter_kernel(RouteArgs a) {
-    constexpr int kEntries = NE < kMostSorted ? NE : kMostSorted;
+    constexpr int kEntries = NE < MOST ? NE : MOST;
     const int token = threadIdx.x >> 4, lane = threadIdx.x & 15;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + token, here = min(t, a.n_tokens - 1);
     float score[NE], value[NE];
@@ -270,7 +281,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_quarter_kernel(RouteArgs
         const int bits = __builtin_bit_cast(int, value[j]);
         entry[j] = __hiloint2double(bits, ~((lane * NE + j) ^ (bits >> 31)));  // (of equal values the one ahead is the larger, of equal negative ones too)
     }
-    sort_best(entry);
+    sort_best<NE, kEntries>(entry);
     int key[kEntries], place[kEntries];
 #pragma unroll
     for (int i = 0; i < kEntries; i++) {
@@ -281,18 +292,19 @@ __global__ __launch_bounds__(256) void moe_route_scored_quarter_kernel(RouteArgs
     const int none = total_key(-INFINITY);
     int where = -1;  // lane s: slot s
 #pragma unroll
-    for (int s = 0; s < kMostSorted; s++) {
+    for (int s = 0; s < MOST; s++) {
         if (s == a.k) break;
         const int m = row_allmax_i32(key[0]);
         const int p = row_allmin_i32(key[0] == m ? place[0] : INT32_MAX);
         where = lane == s && m != none ? p : where;
         const bool next = place[0] == p;
 #pragma unroll
-        for (int i = 0; i < kEntries - 1 && i < kMostSorted - 1 - s; i++) {
-            key[i] = next ? key[i + 1] : key[i];
-            place[i] = next ? place[i + 1] : place[i];
-        }
-        if (s + kEntries < kMostSorted) {
+        for (int i = 0; i < kEntries - 1; i++)
+            if (i < MOST - 1 - s) {  // (what no later turn gets to stays)
+                key[i] = next ? key[i + 1] : key[i];
+                place[i] = next ? place[i + 1] : place[i];
+            }
+        if (s + kEntries < MOST) {
             key[kEntries - 1] = next ? none : key[kEntries - 1];
             place[kEntries - 1] = next ? INT32_MAX : place[kEntries - 1];
         }
@@ -317,12 +329,19 @@ static int launch_route_wave(const RouteArgs &a, hipStream_t st) {
     CML_HIP_TRY(hipGetLastError());
     return CML_OK;
 }
-template <class T, bool SIGMOID, int NE>
+template <class T, bool SIGMOID, int NE, int MOST>
 static int launch_route_quarter(const RouteArgs &a, hipStream_t st) {
     CML_COUNT_LAUNCH("moe.route.scored.quarter");
-    hipLaunchKernelGGL((moe_route_scored_quarter_kernel<T, SIGMOID, NE>), dim3(static_cast<unsigned>((a.n_tokens + 15) / 16)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((moe_route_scored_quarter_kernel<T, SIGMOID, NE, MOST>), dim3(static_cast<unsigned>((a.n_tokens + 15) / 16)), dim3(256), 0, st, a);
     CML_HIP_TRY(hipGetLastError());
     return CML_OK;
+}
+template <class T, bool SIGMOID, int MOST>
+static int launch_route_quarters(const RouteArgs &a, hipStream_t st) {
+    if (a.per <= 4) return launch_route_quarter<T, SIGMOID, 4, MOST>(a, st);
+    if (a.per <= 8) return launch_route_quarter<T, SIGMOID, 8, MOST>(a, st);
+    if (a.per <= 16) return launch_route_quarter<T, SIGMOID, 16, MOST>(a, st);
+    return launch_route_quarter<T, SIGMOID, 32, MOST>(a, st);
 }
 // The groups over the lanes of a token: a power of two lanes each, 16 at most (what rates them stays inside 16 lanes).
 static bool spread_groups(RouteArgs &a, int lanes, int most_per) {
@@ -335,12 +354,10 @@ static bool spread_groups(RouteArgs &a, int lanes, int most_per) {
 }
 template <class T, bool SIGMOID>
 static int launch_route(RouteArgs a, hipStream_t st) {
-    // Four tokens a wave where there are waves enough that way.
-    if (a.n_tokens >= env_int("CAMELID_HIP_ROUTE_QUARTER", 2048) && a.k <= kMostSorted && spread_groups(a, 16, 16)) {
-        if (a.per <= 4) return launch_route_quarter<T, SIGMOID, 4>(a, st);
-        if (a.per <= 8) return launch_route_quarter<T, SIGMOID, 8>(a, st);
-        return launch_route_quarter<T, SIGMOID, 16>(a, st);
-    }
+    // Four tokens a wave where there are waves enough that way (8 of 256 in 8 groups, four against one: 1024 tokens 6.3 and 4.9 us, 4096 6.9 and 7.7, 8192 8.3
+    // and 11.7; 16 of 512, 8192 tokens: 18.5 and 22.8).
+    if (a.n_tokens >= env_int("CAMELID_HIP_ROUTE_QUARTER", 4096) && a.k <= 16 && spread_groups(a, 16, 32))
+        return a.k <= 8 ? launch_route_quarters<T, SIGMOID, 8>(a, st) : launch_route_quarters<T, SIGMOID, 16>(a, st);
     spread_groups(a, 64, 32);  // (1024 experts in up to 64 groups come to 32 a lane at most)
     if (a.per <= 1) return launch_route_wave<T, SIGMOID, 1>(a, st);
     if (a.per <= 2) return launch_route_wave<T, SIGMOID, 2>(a, st);
