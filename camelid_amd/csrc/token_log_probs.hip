@@ -73,14 +73,14 @@ __device__ __forceinline__ void rebase(RowState &s, float most) {
     s.most = most;
 }
 
-// A value that at least n of the 64 K values v are above, close below the n-th largest: bisection over the upper half of the ordered bits.  Where hardly more than
-// n are above `over`, that.
+// A value that at least n of the 64 K values v are above, close below the n-th largest: bisection over the upper half of the ordered bits.  Where no more than
+// `enough` are above `over`, that.
 template <int K>
-__device__ __forceinline__ float below_nth(const float (&v)[K], int n, float over) {
+__device__ __forceinline__ float below_nth(const float (&v)[K], int n, float over, int enough) {
     int above = 0;
 #pragma unroll
     for (int k = 0; k < K; k++) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[k] > over));
-    if (above <= n + 8) return over;  // (the search takes what eight insertions do)
+    if (above <= enough) return over;
     int key[K], low = -32768;
 #pragma unroll
     for (int k = 0; k < K; k++) key[k] = total_key(v[k]) >> 16;
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
         if (!__builtin_amdgcn_ballot_w64(bm > last)) continue;
         // (what the list holds has lower indices than this batch: only larger logits get in)
         const float most[1] = {bm};
-        const float over = below_nth(most, a.n_top, last);
+        const float over = below_nth(most, a.n_top, last, a.n_top + 8);  // (the search takes what eight insertions do)
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (!__builtin_amdgcn_ballot_w64(pm[u] > over)) continue;
@@ -322,7 +322,8 @@ __global__ __launch_bounds__(64) void token_log_probs_join_kernel(ScoreArgs a) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s.above += __shfl_xor(s.above, o);
     if (a.n_top) {
-        float over = below_nth(best, a.n_top, -INFINITY);
+        float over = below_nth(best, a.n_top, -INFINITY, a.n_top + 8);
+        __shared__ uint2 found[64];
         __shared__ int which[kMaxParts];  // the parts that have anything above it
         const unsigned long long first = __builtin_amdgcn_ballot_w64(best[0] > over), second = __builtin_amdgcn_ballot_w64(best[1] > over), below = (1ull << lane) - 1;
         const int n_first = __builtin_popcountll(first), n = (n_first + __builtin_popcountll(second)) * a.n_top;
@@ -340,27 +341,57 @@ __global__ __launch_bounds__(64) void token_log_probs_join_kernel(ScoreArgs a) {
                 v[k] = i < n ? at[0] : -INFINITY;
                 id[k] = __builtin_bit_cast(int, at[a.n_top]);
             }
-            over = below_nth(v, a.n_top, over);
+            over = below_nth(v, a.n_top, over, 64 - a.n_top);
+            int count = 0;
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
-                unsigned long long in = __builtin_amdgcn_ballot_w64(v[k] > over);
-                while (in) {
-                    const int from = __builtin_ctzll(in);
-                    in &= in - 1;
-                    list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[k]), from)), __builtin_amdgcn_readlane(id[k], from));
+                const bool in = v[k] > over;
+                const unsigned long long all = __builtin_amdgcn_ballot_w64(in);
+                const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(all >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(all), 0));
+                if (in && at < 64) found[at] = make_uint2(ordered(__float_as_uint(v[k])), static_cast<uint32_t>(~id[k]));
+                count += __builtin_popcountll(all);
+            }
+            __syncthreads();
+            const int have = min(a.n_top, __builtin_popcountll(__builtin_amdgcn_ballot_w64(s.list != 0)));
+            if (have + count <= 64) {
+                // ranked together with the list, and moved there at once (5 instructions for each, an insertion takes 20)
+                const uint2 next = found[max(lane - have, 0)];
+                uint2 mine = make_uint2(0, 0);
+                if (lane < have) mine = make_uint2(s.list, s.list_low);
+                else if (lane < have + count) mine = next;
+                const uint64_t key = static_cast<uint64_t>(mine.x) << 32 | mine.y;
+                int rank = 0;  // (a lane without an entry: the place behind the last)
+                for (int i = 0; i < have + count; i++) {
+                    const uint64_t other = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(mine.x, i))) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readlane(mine.y, i));
+                    rank += other > key ? 1 : 0;
+                }
+                s.list = __builtin_amdgcn_ds_permute(4 * rank, mine.x);
+                s.list_low = __builtin_amdgcn_ds_permute(4 * rank, mine.y);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) {
+                    unsigned long long in = __builtin_amdgcn_ballot_w64(v[k] > over);
+                    while (in) {
+                        const int from = __builtin_ctzll(in);
+                        in &= in - 1;
+                        list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[k]), from)), __builtin_amdgcn_readlane(id[k], from));
+                    }
                 }
             }
+            __syncthreads();
         }
     }
     write_row<T>(a, row, s, given, in_range, lane);
 }
 
-// Parts per row: 4096 waves for the chip (2048 x 128256 bf16, 20 best: one part a row 134 us, two 127, three 139: every part fills a list of its own), a batch a
-// part at least.  Up to four go into one workgroup, as 1, 2 or 4.
+// Parts per row: 4096 waves for the chip (2048 x 128256 bf16, 20 best: one part a row 134 us, two 121, three 139: every part fills a list of its own), a batch a
+// part at least.  Up to four go into one workgroup, as 1, 2 or 4; four instead of up to eight save the second launch (512 x 32000 f32, 5 best: eight parts 23.8 us,
+// four 18.5; 512 x 128256 bf16, 20 best: 52 either way).  Sixteen waves for a row in one workgroup were slower than two launches: a compute unit takes 4 us for
+// sixteen batches, the second launch 3 to 5.
 static int score_parts(int64_t n_rows, int64_t vocab) {
     const int64_t batches = (vocab + 1023) / 1024;
     const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(env_int("CAMELID_HIP_SCORE_WAVES", 4096) + n_rows - 1) / n_rows, batches, kMaxParts})));
-    return parts == 3 ? 4 : parts;
+    return parts > 2 && parts <= 8 ? 4 : parts;
 }
 
 size_t token_log_probs_workspace(int64_t n_rows, int64_t vocab, int n_top) {

@@ -70,7 +70,7 @@ def test_sizes(t, n, vocab, top, pad, offset):
 
 # parts as long as they can be, a row of one part, and a part a batch
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("waves,vocab", [(1, 60000), (1, 65536), (1, 65537), (1, 200000), (9, 131072), (4096, 30000)])
+@pytest.mark.parametrize("waves,vocab", [(1, 60000), (1, 65536), (1, 65537), (1, 200000), (9, 131072), (4096, 30000), (15, 30000), (16, 70000), (36, 70000), (48, 9000), (45, 100000)])
 def test_rows_cut_otherwise(t, waves, vocab):
     rng = np.random.default_rng(vocab)
     v = (2 * rng.standard_normal((3, vocab))).astype(np.float32)
@@ -162,7 +162,7 @@ def test_on_another_stream_and_replayed_from_a_graph():
 def test_refusals():
     B.init(0)
     L = lib()
-    n, vocab, top = 2, 8192, 4
+    n, vocab, top = 2, 40000, 4
     x, tg = Rows.empty(n, vocab, np.float32), Rows(np.zeros((1, n), np.int32))
     p, r, h, i, a = Rows.empty(1, n, np.float32), Rows.empty(1, n, np.int32), Rows.empty(1, n, np.float32), Rows.empty(n, top, np.int32), Rows.empty(n, top, np.float32)
     need = L.cml_token_log_probs_workspace_bytes(n, vocab, top)
