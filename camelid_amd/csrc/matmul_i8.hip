@@ -706,8 +706,10 @@ int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int
         return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
     }
     CML_COUNT_LAUNCH("i8.matmul.staged");
-    // 128 x 128 where that still is a workgroup for every compute unit
-    const bool large = (rows + 127) / 128 * ((n_tokens + 127) / 128) >= 256;
+    // A step takes a compute unit 0.95 us in the tile of 128 x 128, in those of 64 x 64 0.87 two at a time and 0.48 one alone (rows of 4099, 512 x 4096: 37 and 31 us;
+    // 640 x 4096: 38 and 43; 2048 x 2048: 38 and 55).
+    const int64_t four = (rows + 127) / 128 * ((n_tokens + 127) / 128), one = (rows + 63) / 64 * ((n_tokens + 63) / 64), left = one % 512;
+    const bool large = 0.95f * static_cast<float>((four + 255) / 256) < 0.87f * static_cast<float>(one / 512) + (left > 256 ? 0.87f : left > 0 ? 0.48f : 0.0f);
     return with_type(dtype, [&](auto t) { return large ? launch_staged<decltype(t), 2>(a, st) : launch_staged<decltype(t), 1>(a, st); });
 }
 

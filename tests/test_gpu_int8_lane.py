@@ -211,6 +211,51 @@ def test_scales_that_are_not_finite_reach_their_cells_alone():
     assert np.all(np.isfinite(rest))
 
 
+@pytest.mark.parametrize("tile,n,rows,cols", [(0, 5, 300, 512), (0, 300, 700, 512), (1, 600, 1000, 272), (-1, 70, 90, 272)])
+def test_the_lane_on_a_stream_and_replayed_from_a_graph(tile, n, rows, cols):
+    """Norm and product captured together; every replay on other inputs against the eager calls."""
+    import ctypes as C
+    B.init(0)
+    L, rng = lib(), np.random.default_rng(n)
+    st, graph = C.c_void_p(), C.c_void_p()
+    check(L.cml_stream_create(C.byref(st)))
+    _, w, _, ws, bias = operands(n, 1, rows, cols)
+    sets = [to_bits(rng.standard_normal((n, cols)), "bf16") for _ in range(3)]
+    X, Q, D, O, back = Rows(sets[0]), Rows.empty(n, cols, np.int8), Rows.empty(1, n, np.float32), Rows.empty(n, rows, np.float32), Rows.empty(n, cols, np.uint16)
+    N, W, WS, BI = f32(1 + rng.random(cols)), Rows(w), f32(ws), f32(bias)
+
+    def calls():
+        check(L.cml_add_rms_norm_i8(TYPES["bf16"], X.ptr, cols, None, 0, N.ptr, 1e-6, n, cols, None, 0, None, Q.ptr, cols, D.ptr, st))
+        check(L.cml_matmul_i8(Q.ptr, cols, D.ptr, n, W.ptr, cols, WS.ptr, rows, cols, BI.ptr, 0, O.ptr, rows, st))
+        check(L.cml_dequantize_i8(Q.ptr, cols, D.ptr, n, cols, TYPES["bf16"], back.ptr, cols, st))
+
+    def load(k):
+        check(L.cml_memcpy_h2d(X.ptr, sets[k].ctypes.data, sets[k].nbytes, st))
+
+    def results():
+        check(L.cml_stream_sync(st))
+        return [r.get() for r in (Q, D, O, back)]
+
+    with G.env(CAMELID_HIP_I8_TILE=tile):
+        want = []
+        for k in range(3):
+            load(k)
+            G.say(f"int8 lane {n}x{rows}x{cols} eager {k}")
+            calls()
+            want.append(results())
+        check(L.cml_graph_begin_capture(st))
+        calls()
+        check(L.cml_graph_end_capture(st, C.byref(graph)))
+    for k in (2, 0, 1, 1, 2):
+        load(k)
+        G.say(f"int8 lane {n}x{rows}x{cols} replay {k}")
+        check(L.cml_graph_launch(graph, st))
+        for got, w in zip(results(), want[k]):
+            assert np.array_equal(got, w)
+    check(L.cml_graph_destroy(graph))
+    check(L.cml_stream_destroy(st))
+
+
 def test_refusals():
     B.init(0)
     L = lib()

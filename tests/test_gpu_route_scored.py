@@ -160,6 +160,30 @@ def test_long_prompts(n):
     compare(SIGMOID, "bf16", logits, (rng.integers(-8, 8, 48) / 64.0).astype(np.float32), 4, 2, 2, 6)
 
 
+def test_on_a_stream_and_replayed_from_a_graph():
+    import ctypes as C
+    B.init(0)
+    L, rng = lib(), np.random.default_rng(3)
+    st = C.c_void_p()
+    check(L.cml_stream_create(C.byref(st)))
+    for n in (3, 5000):
+        graph = C.c_void_p()
+        sets = [to_bits(rng.standard_normal((n, 64)), "bf16") for _ in range(2)]
+        want = [route(SIGMOID, "bf16", v, None, 4, 2, 2, 6) for v in sets]
+        X, I, W = Rows(sets[0]), Rows.empty(n, 6, np.int32), Rows.empty(n, 6, np.float32)
+        check(L.cml_graph_begin_capture(st))
+        check(L.cml_moe_route_scored(SIGMOID, TYPES["bf16"], X.ptr, 64, None, n, 64, 4, 2, 2, 6, 1, 1.0, I.ptr, W.ptr, st))
+        check(L.cml_graph_end_capture(st, C.byref(graph)))
+        for k in (1, 0, 1, 1):
+            check(L.cml_memcpy_h2d(X.ptr, sets[k].ctypes.data, sets[k].nbytes, st))
+            G.say(f"moe_route_scored {n} replay {k}")
+            check(L.cml_graph_launch(graph, st))
+            check(L.cml_stream_sync(st))
+            assert np.array_equal(I.get(), want[k][0]) and np.array_equal(W.get(), want[k][1])
+        check(L.cml_graph_destroy(graph))
+    check(L.cml_stream_destroy(st))
+
+
 def test_results_feed_the_plan():
     """Slots without an expert are dropped by the grouping."""
     v = np.full((3, 16), -np.inf, np.float32)
