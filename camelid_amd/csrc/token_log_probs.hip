@@ -40,11 +40,16 @@ __host__ __device__ constexpr int partial_floats(int n_top) { return 5 + 2 * n_t
 // What a wave has seen of a row.  Per lane: most, sum, esum; the same in all lanes: above.
 struct RowState {
     float most = kLowest;   // running maximum, never below the lowest finite value
-    float sum = 0.0f;       // of exp(x - most)
-    float esum = 0.0f;      // of exp(x - most) (x - most) log2(e)
+    float sum = 0.0f;       // of 2^d, d = (x - most) log2(e) + shift(most)
+    float esum = 0.0f;      // of 2^d d
     int above = 0;          // tokens ahead of the given one
     uint32_t list = 0, list_low = 0;  // lane i: the i-th best, by the value's ordered bits, then the inverted id; 0: none
 };
+
+// What rounding most * log2(e) takes off it, for logits of ordinary size.  With it, d is one multiply-add, x log2(e) - rounded(most log2(e)), and as good as from the
+// difference x - most; it goes out of the row's sums at their end.
+constexpr float kOrdinary = 4096.0f;
+__device__ __forceinline__ float shift(float most) { return fabsf(most) < kOrdinary ? fmaf(most, kLog2e, -(most * kLog2e)) : 0.0f; }
 
 // d as a factor: the exponential of one so low is 0, and 0 times a finite number adds nothing (a masked token, an overflowed difference).
 __device__ __forceinline__ float finite_factor(float d) { return fmaxf(d, -1e25f); }
@@ -67,7 +72,7 @@ __device__ __forceinline__ void list_insert(RowState &s, uint32_t v, int id) {
 }
 // The running sums of a lane moved to another maximum.
 __device__ __forceinline__ void rebase(RowState &s, float most) {
-    const float d = (s.most - most) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+    const float d = (s.most - most) * kLog2e + (shift(most) - shift(s.most)), f = __builtin_amdgcn_exp2f(d);
     s.esum = f * fmaf(s.sum, finite_factor(d), s.esum);
     s.sum = f * s.sum;  // (a NaN stays)
     s.most = most;
@@ -103,12 +108,12 @@ __device__ __forceinline__ void close(RowState &s) {
 
 template <class T>
 __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, const RowState &s, float given, bool in_range, int lane) {
-    const float log_sum = __builtin_amdgcn_logf(s.sum) * kLn2;
+    const float all = __builtin_amdgcn_logf(s.sum), log_sum = (all - shift(s.most)) * kLn2;
     const bool empty = s.sum == 0.0f;
     if (lane == 0) {
         a.log_prob[row] = !in_range ? __builtin_nanf("") : empty ? -INFINITY : (given - s.most) - log_sum;
         if (a.rank) a.rank[row] = in_range ? s.above + 1 : 0;
-        if (a.entropy) a.entropy[row] = empty ? 0.0f : log_sum - s.esum / s.sum * kLn2;
+        if (a.entropy) a.entropy[row] = empty ? 0.0f : (all - s.esum / s.sum) * kLn2;
     }
     if (lane < a.n_top) {
         a.top_ids[row * a.n_top + lane] = s.list ? static_cast<int>(~s.list_low) : -1;
@@ -161,6 +166,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
     const float given = in_range ? load_value<T>(x + target) : INFINITY;
     RowState s;
     float last = -INFINITY;  // the list's n-th
+    bool careful = false;    // masked logits were seen
 #pragma unroll 1
     for (int b = begin; b < end; b++) {
         const int base = b * kBatch;
@@ -188,16 +194,41 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
             bm = fmaxf(bm, pm[u]);
         }
         rebase(s, fmaxf(s.most, bm));
+        // (instructions bound a row that comes at memory's rate: one less to a logit, and no clamp, is 2048 x 128256 bf16 in 113 us in place of 122)
+        bool plain = !careful && !__builtin_amdgcn_ballot_w64(!(fabsf(s.most) < kOrdinary));
+        if (plain) {
+            const float from = -(s.most * kLog2e);
+            float sum = s.sum, esum = s.esum;
 #pragma unroll
-        for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float d = (v[u][j] - s.most) * kLog2e, e = __builtin_amdgcn_exp2f(d);
-                s.sum = s.sum + e;
-                s.esum = fmaf(e, finite_factor(d), s.esum);
+                for (int j = 0; j < 8; j++) {
+                    const float d = fmaf(v[u][j], kLog2e, from), e = __builtin_amdgcn_exp2f(d);
+                    sum = sum + e;
+                    esum = fmaf(e, d, esum);
+                }
+            careful = __builtin_amdgcn_ballot_w64(esum != esum) != 0;  // a masked logit (0 times -inf), or a NaN: this batch again, and the rest of the part so
+            plain = !careful;
+            if (plain) {
+                s.sum = sum;
+                s.esum = esum;
             }
-        // tokens ahead of the given one: of equal logits those with a lower index
-        if (whole && base + kBatch <= target) {
+        }
+        if (!plain) {
+            const float more = shift(s.most);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float d = (v[u][j] - s.most) * kLog2e + more, e = __builtin_amdgcn_exp2f(d);
+                    s.sum = s.sum + e;
+                    s.esum = fmaf(e, finite_factor(d), s.esum);
+                }
+        }
+        // tokens ahead of the given one: of equal logits those with a lower index (a given token is mostly among the first, and a batch without any ahead of it is
+        // passed over)
+        if (!__builtin_amdgcn_ballot_w64(bm >= given)) {
+        } else if (whole && base + kBatch <= target) {
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll

@@ -90,6 +90,18 @@ def test_orders_and_ties(t, kind):
     compare(t, rows, np.array([0, vocab - 1, 4321, 1024]), top)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_logits_of_any_size(t):
+    """Large ones beside ordinary ones, in either order, of both signs; some of them masked later on."""
+    vocab, rng = 9000, np.random.default_rng(9)
+    small, up = rng.standard_normal(vocab), np.linspace(-30, 12000, vocab)
+    v = np.stack([up, up[::-1], 4090 + 4 * small, -5000 + 4 * small, 60 + small, np.where(np.arange(vocab) % 4097 == 0, 20000.0, small), 1000 + small, 4096 * np.sign(small), small * 1e-6])
+    v[6, 5000:8000] = -np.inf
+    v[4, 8191] = -np.inf
+    v[8, 100:300] = -np.inf
+    compare(t, to_bits(v.astype(np.float32), t), rng.integers(vocab, size=len(v)), 20)
+
+
 def test_signed_zeros_tie():
     v = np.zeros((1, 3000), np.float32)
     v[0, ::2] = -0.0
