@@ -8,7 +8,10 @@
 // row are joined inside the workgroup where it has them all, else by a second launch.
 //
 // Logits are looked at one by one for the list only where a batch holds one above the list's last.  Where it holds many (the first one; ascending
-// logits), a bisection over the lanes' maxima first finds a value that at least n of the batch reach.
+// logits), a bisection over the lanes' maxima first finds a value that at least n of the batch reach, and one over all its logits where that leaves too many.
+//
+// Rows are to be read once, at memory's rate: 2048 x 128256 bf16 in 95 us without a list (5.5 TB/s), 113 with 20 best; what bounds the latter is instruction issue, 12
+// to a logit and 80 insertions a part.  One row of 128256 f32 and 20 best: 10.9 us, two launches of which each waits for memory once.
 //
 // -inf is a masked token: probability 0, no alternative.  A row of nothing else has log probability -inf, entropy 0 and no alternatives.  NaN or +inf in a
 // row leaves NaN in log probability and entropy, as the formula does.  A row at the type's lowest value is an ordinary, uniform row.
@@ -23,6 +26,7 @@ namespace cml {
 constexpr float kLowest = -3.4028235e38f;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kMaxParts = 128;  // per row: two for a lane of the joining wave
+constexpr int kJoinThreads = 512;
 
 struct ScoreArgs {
     const void *logits;
@@ -32,9 +36,10 @@ struct ScoreArgs {
     float *partial;
     int64_t stride, n_rows;
     int vocab, n_top, parts;
+    uint32_t top_inverse;  // ceil(2^20 / n_top): i / n_top = i * top_inverse >> 20 for i < 8192
 };
 
-// most, sum, esum, above, the given logit; the list's values, its ids
+// most, sum, esum, above, the given logit; the list, value and id by turns
 __host__ __device__ constexpr int partial_floats(int n_top) { return 5 + 2 * n_top; }
 
 // What a wave has seen of a row.  Per lane: most, sum, esum; the same in all lanes: above.
@@ -70,6 +75,17 @@ __device__ __forceinline__ void list_insert(RowState &s, uint32_t v, int id) {
     s.list = stays ? s.list : after ? v : up;
     s.list_low = stays ? s.list_low : after ? static_cast<uint32_t>(~id) : up_low;
 }
+// The list from entries in any order, one a lane, `count` of them in the first lanes and 0 behind: each goes to the place that the number of larger ones says.
+__device__ __forceinline__ void list_rank(RowState &s, uint2 mine, int count) {
+    const uint64_t key = static_cast<uint64_t>(mine.x) << 32 | mine.y;
+    int rank = 0;  // (a lane without an entry: the place behind the last)
+    for (int i = 0; i < count; i++) {
+        const uint64_t other = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(mine.x, i))) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readlane(mine.y, i));
+        rank += other > key ? 1 : 0;
+    }
+    s.list = __builtin_amdgcn_ds_permute(4 * rank, mine.x);
+    s.list_low = __builtin_amdgcn_ds_permute(4 * rank, mine.y);
+}
 // The running sums of a lane moved to another maximum.
 __device__ __forceinline__ void rebase(RowState &s, float most) {
     const float d = (s.most - most) * kLog2e + (shift(most) - shift(s.most)), f = __builtin_amdgcn_exp2f(d);
@@ -78,25 +94,38 @@ __device__ __forceinline__ void rebase(RowState &s, float most) {
     s.most = most;
 }
 
-// A value that at least n of the 64 K values v are above, close below the n-th largest: bisection over the upper half of the ordered bits.  Where no more than
-// `enough` are above `over`, that.
+// How many of the 64 K values v are above x.
 template <int K>
-__device__ __forceinline__ float below_nth(const float (&v)[K], int n, float over, int enough) {
+__device__ __forceinline__ int count_above(const float (&v)[K], float x) {
     int above = 0;
 #pragma unroll
-    for (int k = 0; k < K; k++) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[k] > over));
-    if (above <= enough) return over;
-    int key[K], low = -32768;
+    for (int k = 0; k < K; k++) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[k] > x));
+    return above;
+}
+// A value that at least n of them are above, close below the n-th largest: bisection over the upper half of the ordered bits.  At least n have to be above -inf.
+template <int K>
+__device__ __forceinline__ float below_nth(const float (&v)[K], int n) {
+    int low = -32768;
+    const auto under = [](int half) __attribute__((always_inline)) {
+        const int key = static_cast<int>(static_cast<unsigned>(half) << 16) - 1;
+        return from_total_key(key == -1 ? -2 : key);  // (-0 is not below 0)
+    };
+    if constexpr (K <= 2) {
+        int key[K];
 #pragma unroll
-    for (int k = 0; k < K; k++) key[k] = total_key(v[k]) >> 16;
-    for (int bit = 32768; bit; bit >>= 1) {
-        int reach = 0;
+        for (int k = 0; k < K; k++) key[k] = total_key(v[k]) >> 16;
+        for (int bit = 32768; bit; bit >>= 1) {
+            int reach = 0;
 #pragma unroll
-        for (int k = 0; k < K; k++) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] >= low + bit));
-        if (reach >= n) low += bit;
+            for (int k = 0; k < K; k++) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] >= low + bit));
+            if (reach >= n) low += bit;
+        }
+    } else {
+#pragma unroll 1
+        for (int bit = 32768; bit; bit >>= 1)
+            if (count_above(v, under(low + bit)) >= n) low += bit;  // (past the infinities: NaN, above which is nothing)
     }
-    const int under = static_cast<int>(static_cast<unsigned>(low) << 16) - 1;
-    return fmaxf(over, from_total_key(under == -1 ? -2 : under));  // (-0 is not below 0)
+    return under(low);
 }
 
 // Sums over the lanes, every lane at the row's maximum.
@@ -150,6 +179,7 @@ struct Batch {
 template <class T, bool INSIDE>
 __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
     typedef typename T::Bits Bits;
+    __shared__ uint2 found[INSIDE ? 1 : 4][64];
     constexpr int U = Batch<T>::kPieces, kBatch = Batch<T>::kLogits;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t id = blockIdx.x * 4 + wave, row = id / static_cast<uint32_t>(a.parts), part = id - row * a.parts;
@@ -251,7 +281,41 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
         if (!__builtin_amdgcn_ballot_w64(bm > last)) continue;
         // (what the list holds has lower indices than this batch: only larger logits get in)
         const float most[1] = {bm};
-        const float over = below_nth(most, a.n_top, last, a.n_top + 8);  // (the search takes what eight insertions do)
+        float over = last;
+        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(bm > over)) > a.n_top + 8) over = fmaxf(over, below_nth(most, a.n_top));  // (the search takes what eight insertions do)
+        const int lanes = __builtin_popcountll(__builtin_amdgcn_ballot_w64(bm > over));
+        if (!whole || lanes >= 32) {  // lanes with many above it: a search among all of them takes what 80 insertions do
+            const float (&all)[8 * U] = *reinterpret_cast<const float(*)[8 * U]>(&v);
+            if (count_above(all, over) > (INSIDE ? a.n_top + 80 : 64)) over = fmaxf(over, below_nth(all, a.n_top));
+        }
+        if (!INSIDE && lanes > 12) {
+            // Few rows, and the wave has the unit to itself: an insertion takes 60 ns, one after the other; gathered and ranked at once, 28 are 0.9 us instead of 1.7.
+            int count = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (!__builtin_amdgcn_ballot_w64(pm[u] > over)) continue;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const bool in = v[u][j] > over;
+                    const unsigned long long those = __builtin_amdgcn_ballot_w64(in);
+                    const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(those >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(those), 0));
+                    if (in && at < 64) found[wave][at] = make_uint2(ordered(__float_as_uint(v[u][j])), static_cast<uint32_t>(~(base + (u * 64 + lane) * 8 + j)));
+                    count += __builtin_popcountll(those);
+                }
+            }
+            const int have = min(a.n_top, __builtin_popcountll(__builtin_amdgcn_ballot_w64(s.list != 0)));
+            if (have + count <= 64) {
+                __builtin_amdgcn_wave_barrier();
+                const uint2 next = found[wave][max(lane - have, 0)];
+                __builtin_amdgcn_wave_barrier();
+                uint2 mine = make_uint2(0, 0);
+                if (lane < have) mine = make_uint2(s.list, s.list_low);
+                else if (lane < have + count) mine = next;
+                list_rank(s, mine, have + count);
+                last = from_ordered(__builtin_amdgcn_readlane(s.list, a.n_top - 1));
+                continue;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (!__builtin_amdgcn_ballot_w64(pm[u] > over)) continue;
@@ -315,101 +379,94 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
             p[4] = given;
         }
         if (lane < a.n_top) {
-            p[5 + lane] = from_ordered(s.list);
-            p[5 + a.n_top + lane] = __uint_as_float(~s.list_low);
+            p[5 + 2 * lane] = from_ordered(s.list);
+            p[6 + 2 * lane] = __uint_as_float(~s.list_low);
         }
     }
 }
 
-// The parts of a row, joined by one wave, lane p taking parts p and p + 64.  Of the lists only what reaches the n-th largest of the parts' best is looked at.
+// The parts of a row, joined: every thread asks for its share of the lists and every wave for the parts' best at once, so that memory is waited for once.  What
+// reaches the n-th largest of the parts' best is gathered in LDS and ranked there (3 instructions for each, an insertion takes 20); the first wave adds the sums up
+// (lane p: parts p and p + 64) and writes.  One row of 126 parts: 5 us with 20 best, 2.6 without a list, most of it the launch and the trip.
 template <class T>
-__global__ __launch_bounds__(64) void token_log_probs_join_kernel(ScoreArgs a) {
-    const int lane = threadIdx.x;
+__global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(ScoreArgs a) {
+    __shared__ uint2 found[kJoinThreads], sorted[64];
+    __shared__ int n_found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t row = blockIdx.x;
-    const int width = partial_floats(a.n_top);
+    const int width = partial_floats(a.n_top), n = a.parts * a.n_top;
     const float *rows = a.partial + row * a.parts * width;
+    typedef uint32_t v2u __attribute__((ext_vector_type(2), aligned(4)));
+    const auto entry = [&](int i) __attribute__((always_inline)) {
+        const int part = static_cast<int>(static_cast<uint32_t>(i) * a.top_inverse >> 20);
+        return *reinterpret_cast<const v2u *>(rows + part * width + 5 + 2 * (i - part * a.n_top));
+    };
+    constexpr int kMine = kMaxParts * 64 / kJoinThreads;
+    v2u mine[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; k++)
+        if (k * kJoinThreads < n) mine[k] = entry(min(k * kJoinThreads + tid, n - 1));
+    const float *p[2] = {rows + min(lane, a.parts - 1) * width, rows + min(lane + 64, a.parts - 1) * width};
+    const bool here[2] = {lane < a.parts, lane + 64 < a.parts};
+    float over = -INFINITY;
+    if (a.n_top) {
+        const float best[2] = {here[0] ? p[0][5] : -INFINITY, here[1] ? p[1][5] : -INFINITY};
+        if (tid == 0) n_found = 0;
+        if (count_above(best, -INFINITY) > a.n_top) over = below_nth(best, a.n_top);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kMine; k++)
+            if (k * kJoinThreads < n && k * kJoinThreads + tid < n && __uint_as_float(mine[k][0]) > over) {
+                const int at = atomicAdd(&n_found, 1);  // (in any order: the ranks are the same)
+                if (at < kJoinThreads) found[at] = make_uint2(ordered(mine[k][0]), ~mine[k][1]);
+            }
+        __syncthreads();
+        if (64 * wave < n_found && n_found <= kJoinThreads) {
+            const uint2 own = tid < n_found ? found[tid] : make_uint2(0, 0);
+            const uint64_t key = static_cast<uint64_t>(own.x) << 32 | own.y;
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < n_found; i++) rank += (static_cast<uint64_t>(found[i].x) << 32 | found[i].y) > key ? 1 : 0;
+            if (tid < n_found && rank < 64) sorted[rank] = own;
+        }
+        __syncthreads();
+    }
+    if (wave > 0) return;
     const int target = a.target[row];
     const bool in_range = target >= 0 && target < a.vocab;
     const float given = rows[4];
     RowState s;
-    float best[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const bool here = lane + 64 * k < a.parts;
-        const float *p = rows + min(lane + 64 * k, a.parts - 1) * width;
         RowState o;
-        o.most = here ? p[0] : kLowest;
-        o.sum = here ? p[1] : 0.0f;
-        o.esum = here ? p[2] : 0.0f;
-        best[k] = here && a.n_top ? p[5] : -INFINITY;
+        o.most = here[k] ? p[k][0] : kLowest;
+        o.sum = here[k] ? p[k][1] : 0.0f;
+        o.esum = here[k] ? p[k][2] : 0.0f;
         const float most = fmaxf(s.most, o.most);
         rebase(s, most);
         rebase(o, most);
         s.sum = s.sum + o.sum;
         s.esum = s.esum + o.esum;
-        s.above += here ? __builtin_bit_cast(int, p[3]) : 0;
+        s.above += here[k] ? __builtin_bit_cast(int, p[k][3]) : 0;
     }
     close(s);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s.above += __shfl_xor(s.above, o);
     if (a.n_top) {
-        float over = below_nth(best, a.n_top, -INFINITY, a.n_top + 8);
-        __shared__ uint2 found[64];
-        __shared__ int which[kMaxParts];  // the parts that have anything above it
-        const unsigned long long first = __builtin_amdgcn_ballot_w64(best[0] > over), second = __builtin_amdgcn_ballot_w64(best[1] > over), below = (1ull << lane) - 1;
-        const int n_first = __builtin_popcountll(first), n = (n_first + __builtin_popcountll(second)) * a.n_top;
-        if (best[0] > over) which[__builtin_popcountll(first & below)] = lane;
-        if (best[1] > over) which[n_first + __builtin_popcountll(second & below)] = lane + 64;
-        __syncthreads();
-        constexpr int kAhead = 8;
-        for (int i0 = 0; i0 < n; i0 += 64 * kAhead) {
-            float v[kAhead];
-            int id[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                const int i = i0 + 64 * k + lane, nth = min(i, n - 1) / a.n_top;
-                const float *at = rows + which[nth] * width + 5 + min(i, n - 1) - nth * a.n_top;
-                v[k] = i < n ? at[0] : -INFINITY;
-                id[k] = __builtin_bit_cast(int, at[a.n_top]);
-            }
-            over = below_nth(v, a.n_top, over, 64 - a.n_top);
-            int count = 0;
-#pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                const bool in = v[k] > over;
-                const unsigned long long all = __builtin_amdgcn_ballot_w64(in);
-                const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(all >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(all), 0));
-                if (in && at < 64) found[at] = make_uint2(ordered(__float_as_uint(v[k])), static_cast<uint32_t>(~id[k]));
-                count += __builtin_popcountll(all);
-            }
-            __syncthreads();
-            const int have = min(a.n_top, __builtin_popcountll(__builtin_amdgcn_ballot_w64(s.list != 0)));
-            if (have + count <= 64) {
-                // ranked together with the list, and moved there at once (5 instructions for each, an insertion takes 20)
-                const uint2 next = found[max(lane - have, 0)];
-                uint2 mine = make_uint2(0, 0);
-                if (lane < have) mine = make_uint2(s.list, s.list_low);
-                else if (lane < have + count) mine = next;
-                const uint64_t key = static_cast<uint64_t>(mine.x) << 32 | mine.y;
-                int rank = 0;  // (a lane without an entry: the place behind the last)
-                for (int i = 0; i < have + count; i++) {
-                    const uint64_t other = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(mine.x, i))) << 32 | static_cast<uint32_t>(__builtin_amdgcn_readlane(mine.y, i));
-                    rank += other > key ? 1 : 0;
+        if (n_found <= kJoinThreads) {
+            s.list = lane < n_found ? sorted[lane].x : 0;
+            s.list_low = lane < n_found ? sorted[lane].y : 0;
+        } else {  // many alike, or the best side by side: one after the other
+            for (int i0 = 0; i0 < n; i0 += 64) {
+                const v2u e = entry(min(i0 + lane, n - 1));
+                unsigned long long in = __builtin_amdgcn_ballot_w64(i0 + lane < n && __uint_as_float(e[0]) > over);
+                while (in) {
+                    const int from = __builtin_ctzll(in);
+                    in &= in - 1;
+                    list_insert(s, ordered(__builtin_amdgcn_readlane(e[0], from)), __builtin_amdgcn_readlane(e[1], from));
                 }
-                s.list = __builtin_amdgcn_ds_permute(4 * rank, mine.x);
-                s.list_low = __builtin_amdgcn_ds_permute(4 * rank, mine.y);
-            } else {
-#pragma unroll
-                for (int k = 0; k < kAhead; k++) {
-                    unsigned long long in = __builtin_amdgcn_ballot_w64(v[k] > over);
-                    while (in) {
-                        const int from = __builtin_ctzll(in);
-                        in &= in - 1;
-                        list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[k]), from)), __builtin_amdgcn_readlane(id[k], from));
-                    }
-                }
+                over = fmaxf(over, from_ordered(__builtin_amdgcn_readlane(s.list, a.n_top - 1)));
             }
-            __syncthreads();
         }
     }
     write_row<T>(a, row, s, given, in_range, lane);
@@ -432,7 +489,8 @@ size_t token_log_probs_workspace(int64_t n_rows, int64_t vocab, int n_top) {
 
 int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_t n_rows, int64_t vocab, const int32_t *target, int n_top, float *log_prob, int32_t *rank, float *entropy,
                            int32_t *top_ids, float *top_log_probs, void *workspace, hipStream_t st) {
-    const ScoreArgs a{logits, target, log_prob, entropy, top_log_probs, rank, top_ids, static_cast<float *>(workspace), stride, n_rows, static_cast<int>(vocab), n_top, score_parts(n_rows, vocab)};
+    const ScoreArgs a{logits, target, log_prob, entropy, top_log_probs, rank, top_ids, static_cast<float *>(workspace), stride, n_rows, static_cast<int>(vocab), n_top, score_parts(n_rows, vocab),
+                      n_top ? ((1u << 20) + n_top - 1) / n_top : 0};
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         const dim3 grid(static_cast<unsigned>((n_rows * a.parts + 3) / 4));
@@ -442,7 +500,7 @@ int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_
         } else {
             CML_COUNT_LAUNCH("score.parts");
             hipLaunchKernelGGL((token_log_probs_kernel<T, false>), grid, dim3(256), 0, st, a);
-            hipLaunchKernelGGL(token_log_probs_join_kernel<T>, dim3(static_cast<unsigned>(n_rows)), dim3(64), 0, st, a);
+            hipLaunchKernelGGL(token_log_probs_join_kernel<T>, dim3(static_cast<unsigned>(n_rows)), dim3(kJoinThreads), 0, st, a);
         }
         CML_HIP_TRY(hipGetLastError());
         return CML_OK;

@@ -102,6 +102,23 @@ def test_logits_of_any_size(t):
     compare(t, to_bits(v.astype(np.float32), t), rng.integers(vocab, size=len(v)), 20)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [20, 33, 64])
+def test_the_best_side_by_side(t, top):
+    """All of them in the last part, in the first one, and in a few parts; alike in value."""
+    vocab = 150000
+    up = np.linspace(-20, 20, vocab)
+    few = np.where(np.arange(vocab) % 30000 < 40, 9.0, 0.0) + np.arange(vocab) % 7 / 8
+    compare(t, to_bits(np.stack([up, up[::-1], few, np.zeros(vocab)]).astype(np.float32), t), np.array([0, 149999, 70000, 5]), top)
+
+
+@pytest.mark.parametrize("vocab", [1025, 1200, 1280, 2303])
+@pytest.mark.parametrize("top", [24, 40, 64])
+def test_lists_longer_than_a_short_last_batch(vocab, top):
+    v = np.random.default_rng(vocab).standard_normal((70, vocab)).astype(np.float32)
+    compare("f32", v.view(np.uint32), np.zeros(70, int), top)
+
+
 def test_signed_zeros_tie():
     v = np.zeros((1, 3000), np.float32)
     v[0, ::2] = -0.0
