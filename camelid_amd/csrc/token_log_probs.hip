@@ -226,9 +226,9 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
         rebase(s, fmaxf(s.most, bm));
         // (instructions bound a row that comes at memory's rate: one less to a logit, and no clamp, is 2048 x 128256 bf16 in 113 us in place of 122)
         bool plain = !careful && !__builtin_amdgcn_ballot_w64(!(fabsf(s.most) < kOrdinary));
+        float sum = 0.0f, esum = 0.0f;  // (of this batch: a row's sum is one of few large terms)
         if (plain) {
             const float from = -(s.most * kLog2e);
-            float sum = s.sum, esum = s.esum;
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
@@ -239,22 +239,21 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
                 }
             careful = __builtin_amdgcn_ballot_w64(esum != esum) != 0;  // a masked logit (0 times -inf), or a NaN: this batch again, and the rest of the part so
             plain = !careful;
-            if (plain) {
-                s.sum = sum;
-                s.esum = esum;
-            }
         }
         if (!plain) {
             const float more = shift(s.most);
+            sum = esum = 0.0f;
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float d = (v[u][j] - s.most) * kLog2e + more, e = __builtin_amdgcn_exp2f(d);
-                    s.sum = s.sum + e;
-                    s.esum = fmaf(e, finite_factor(d), s.esum);
+                    sum = sum + e;
+                    esum = fmaf(e, finite_factor(d), esum);
                 }
         }
+        s.sum = s.sum + sum;
+        s.esum = s.esum + esum;
         // tokens ahead of the given one: of equal logits those with a lower index (a given token is mostly among the first, and a batch without any ahead of it is
         // passed over)
         if (!__builtin_amdgcn_ballot_w64(bm >= given)) {
@@ -472,14 +471,14 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Scor
     write_row<T>(a, row, s, given, in_range, lane);
 }
 
-// Parts per row: 4096 waves for the chip (2048 x 128256 bf16, 20 best: one part a row 134 us, two 121, three 139: every part fills a list of its own), a batch a
-// part at least.  Up to four go into one workgroup, as 1, 2 or 4; four instead of up to eight save the second launch (512 x 32000 f32, 5 best: eight parts 23.8 us,
-// four 18.5; 512 x 128256 bf16, 20 best: 52 either way).  Sixteen waves for a row in one workgroup were slower than two launches: a compute unit takes 4 us for
-// sixteen batches, the second launch 3 to 5.
+// Parts per row: up to 4096 waves, which the chip holds at once (2048 x 128256 bf16, 20 best: one part a row 130 us, two 113, four 130, every part filling a list of its
+// own; 1500 rows: one 130, two 97, four 105; 3000: one 160, two 170), a batch a part at least.  Up to four go into one workgroup, as 1, 2 or 4; four instead of up to
+// eight save the second launch (512 x 32000 f32, 5 best: eight 23.8 us, four 18.5; 512 x 128256 bf16, 20 best: 52 either way).  Sixteen waves for a row in one workgroup
+// were slower than two launches: a compute unit takes 4 us for sixteen batches, the second launch 3 to 5.
 static int score_parts(int64_t n_rows, int64_t vocab) {
     const int64_t batches = (vocab + 1023) / 1024;
-    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(env_int("CAMELID_HIP_SCORE_WAVES", 4096) + n_rows - 1) / n_rows, batches, kMaxParts})));
-    return parts > 2 && parts <= 8 ? 4 : parts;
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({env_int("CAMELID_HIP_SCORE_WAVES", 4096) / std::max<int64_t>(1, n_rows), batches, kMaxParts})));
+    return parts >= 4 && parts <= 8 ? 4 : parts == 3 ? 2 : parts;
 }
 
 size_t token_log_probs_workspace(int64_t n_rows, int64_t vocab, int n_top) {
