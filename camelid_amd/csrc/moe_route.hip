@@ -10,8 +10,9 @@
 // An expert whose logit is NaN or -inf, or whose key is, takes no part; a token left with fewer than k experts has id -1 and weight 0 in the slots behind
 // them (the expert lane drops such slots).  +inf counts as the largest finite logit.
 //
-// A token has a whole wave, or 16 lanes of one.  A group has 1, 2, 4, 8 or 16 lanes and each of them `per` neighbouring experts (the group's last one maybe
-// fewer): what is ahead in lane and place has the lower index.
+// A token has a whole wave, or 16 lanes of one.  A group has 1, 2, 4, 8 or 16 lanes and each of them NE neighbouring experts (the group's last ones fewer or none):
+// what is ahead in lane and place has the lower index.  With 16 lanes for a token each has the experts of four, and adds them up as four, so that both forms give the
+// same bits.
 #include <type_traits>
 
 #include "typed_rows.hpp"
@@ -29,7 +30,6 @@ struct RouteArgs {
     int n_experts, n_groups, groups_kept, group_top, k;
     int group_size;
     int group_shift;  // log2 of the lanes that hold a group
-    int per;          // experts per lane
     int renormalise;
     float weight_scale;
 };
@@ -37,18 +37,19 @@ struct RouteArgs {
 constexpr int kOut = INT32_MIN;  // key of an expert that takes no part: below every ordered float
 
 // The experts of a lane.
+template <int NE>
 struct LaneExperts {
     int first, count;
     __device__ __forceinline__ LaneExperts(const RouteArgs &a, int lane) {
-        const int group = lane >> a.group_shift, at = (lane & ((1 << a.group_shift) - 1)) * a.per;
+        const int group = lane >> a.group_shift, at = (lane & ((1 << a.group_shift) - 1)) * NE;
         first = group * a.group_size + at;
-        count = group < a.n_groups ? max(0, min(a.per, a.group_size - at)) : 0;
+        count = group < a.n_groups ? max(0, min(NE, a.group_size - at)) : 0;
     }
 };
 
 // Their values, -inf behind the last.
 template <class T, int NE>
-__device__ __forceinline__ void load_experts(const typename T::Bits *p, const LaneExperts &my, float (&v)[NE]) {
+__device__ __forceinline__ void load_experts(const typename T::Bits *p, const LaneExperts<NE> &my, float (&v)[NE]) {
     if constexpr (NE >= 8) {
         if (my.count == NE) {
 #pragma unroll
@@ -73,7 +74,7 @@ __device__ __forceinline__ void load_experts(const typename T::Bits *p, const La
 
 // Scores and values (the floats behind the keys) of a lane's experts; LANES lanes have the token.  in: takes part; the value of one that does not is -inf.
 template <class T, bool SIGMOID, int NE, int LANES>
-__device__ __forceinline__ void rate_experts(const RouteArgs &a, int64_t t, const LaneExperts &my, float (&score)[NE], float (&value)[NE], bool (&in)[NE]) {
+__device__ __forceinline__ void rate_experts(const RouteArgs &a, int64_t t, const LaneExperts<NE> &my, float (&score)[NE], float (&value)[NE], bool (&in)[NE]) {
     float most = -3.4028235e38f;
     load_experts<T, NE>(static_cast<const typename T::Bits *>(a.logits) + t * a.stride, my, value);
 #pragma unroll
@@ -87,13 +88,16 @@ __device__ __forceinline__ void rate_experts(const RouteArgs &a, int64_t t, cons
         for (int j = 0; j < NE; j++) score[j] = in[j] ? 1.0f / (1.0f + expf(-value[j])) : 0.0f;
     } else {
         most = from_total_key(LANES == 64 ? wave_allmax_i32(total_key(most)) : row_allmax_i32(total_key(most)));
-        float sum = 0.0f;
+        constexpr int kParts = 64 / LANES;
+        float sum[kParts] = {};
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             score[j] = in[j] ? expf(value[j] - most) : 0.0f;
-            sum = sum + score[j];
+            sum[j / (NE / kParts)] = sum[j / (NE / kParts)] + score[j];
         }
-        const float total = LANES == 64 ? wave_allsum(sum) : row_allsum(sum);
+        float total;
+        if constexpr (LANES == 64) total = rows_allsum(sum[0]);
+        else total = row_allsum((sum[0] + sum[1]) + (sum[2] + sum[3]));
         if (total > 0.0f)
 #pragma unroll
             for (int j = 0; j < NE; j++) score[j] = score[j] / total;
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
     if (t >= a.n_tokens) return;  // (a wave's work is its own: no barriers)
     float score[NE], value[NE];
     bool in[NE];
-    const LaneExperts my(a, lane);
+    const LaneExperts<NE> my(a, lane);
     rate_experts<T, SIGMOID, NE, 64>(a, t, my, score, value, in);
     int key[NE];
 #pragma unroll
@@ -188,7 +192,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
     }
     // the chosen experts and their scores, from the lanes that hold them
     const int holder = (place < 0 ? 0 : place) / NE;
-    const int chosen = place < 0 ? -1 : LaneExperts(a, holder).first + place % NE;
+    const int chosen = place < 0 ? -1 : LaneExperts<NE>(a, holder).first + place % NE;
     float w = 0.0f;
 #pragma unroll
     for (int j = 0; j < NE; j++) {
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
         w = place >= 0 && place % NE == j ? theirs : w;
     }
     if (a.renormalise) {
-        const float sum = wave_allsum(w);
+        const float sum = rows_allsum(w);
         const int live = __builtin_popcountll(__builtin_amdgcn_ballot_w64(chosen >= 0));
         w = sum > 0.0f ? w / sum : chosen >= 0 ? 1.0f / static_cast<float>(live) : 0.0f;  // (all chosen scores 0: alike)
     }
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
 // Four tokens a wave, 16 lanes each, for up to MOST of 16 * NE experts.  Every lane sorts its experts first, as doubles: a value's f32 bits are the upper word (finite
 // and infinite floats are finite doubles, in the same order), its place the lower one, so that a comparison that the chip makes at full rate decides ties as well.
 // Then the lanes' first entries meet k times, and the lane that held the best goes on to its next.  A turn's
-// maximum over 16 lanes serves four tokens, so a token takes 250 instructions in place of 600: 8 of 256 for 8192 tokens 8.3 us, two waves to a SIMD and bound by the
+// maximum over 16 lanes serves four tokens, so a token takes 340 instructions in place of some 600: 8 of 256 for 8192 tokens 8.4 us, two waves to a SIMD and bound by the
 // latency of their chains.
 __device__ __forceinline__ void sort_two(double &a, double &b) {  // descending
     const double hi = __builtin_fmax(a, b);
@@ -257,7 +261,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_quarter_kernel(RouteArgs
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 16 + token, here = min(t, a.n_tokens - 1);
     float score[NE], value[NE];
     bool in[NE];
-    const LaneExperts my(a, lane);
+    const LaneExperts<NE> my(a, lane);
     rate_experts<T, SIGMOID, NE, 16>(a, here, my, score, value, in);
     __shared__ __align__(16) float scores[16][16 * NE];  // (written and read by the same wave)
 #pragma unroll
@@ -309,7 +313,7 @@ __global__ __launch_bounds__(256) void moe_route_scored_quarter_kernel(RouteArgs
             place[kEntries - 1] = next ? INT32_MAX : place[kEntries - 1];
         }
     }
-    const int chosen = where < 0 ? -1 : LaneExperts(a, where / NE).first + where % NE;
+    const int chosen = where < 0 ? -1 : LaneExperts<NE>(a, where / NE).first + where % NE;
     float w = where >= 0 ? scores[token][where] : 0.0f;
     if (a.renormalise) {
         const float sum = row_allsum(w);
@@ -337,40 +341,38 @@ static int launch_route_quarter(const RouteArgs &a, hipStream_t st) {
     return CML_OK;
 }
 template <class T, bool SIGMOID, int MOST>
-static int launch_route_quarters(const RouteArgs &a, hipStream_t st) {
-    if (a.per <= 4) return launch_route_quarter<T, SIGMOID, 4, MOST>(a, st);
-    if (a.per <= 8) return launch_route_quarter<T, SIGMOID, 8, MOST>(a, st);
-    if (a.per <= 16) return launch_route_quarter<T, SIGMOID, 16, MOST>(a, st);
+static int launch_route_quarters(const RouteArgs &a, int ne, hipStream_t st) {
+    if (ne == 4) return launch_route_quarter<T, SIGMOID, 4, MOST>(a, st);
+    if (ne == 8) return launch_route_quarter<T, SIGMOID, 8, MOST>(a, st);
+    if (ne == 16) return launch_route_quarter<T, SIGMOID, 16, MOST>(a, st);
     return launch_route_quarter<T, SIGMOID, 32, MOST>(a, st);
-}
-// The groups over the lanes of a token: a power of two lanes each, 16 at most (what rates them stays inside 16 lanes).
-static bool spread_groups(RouteArgs &a, int lanes, int most_per) {
-    if (a.n_groups > lanes) return false;
-    int shift = 0;
-    while (a.n_groups << (shift + 1) <= lanes && (shift < 4 || a.n_groups == 1)) shift++;
-    a.group_shift = shift;
-    a.per = (a.group_size + (1 << shift) - 1) >> shift;
-    return a.per <= most_per;
 }
 template <class T, bool SIGMOID>
 static int launch_route(RouteArgs a, hipStream_t st) {
-    // Four tokens a wave where there are waves enough that way (8 of 256 in 8 groups, four against one: 1024 tokens 6.3 and 4.9 us, 4096 6.9 and 7.7, 8192 8.3
-    // and 11.7; 16 of 512, 8192 tokens: 18.5 and 22.8).
-    if (a.n_tokens >= env_int("CAMELID_HIP_ROUTE_QUARTER", 4096) && a.k <= 16 && spread_groups(a, 16, 32))
-        return a.k <= 8 ? launch_route_quarters<T, SIGMOID, 8>(a, st) : launch_route_quarters<T, SIGMOID, 16>(a, st);
-    spread_groups(a, 64, 32);  // (1024 experts in up to 64 groups come to 32 a lane at most)
-    if (a.per <= 1) return launch_route_wave<T, SIGMOID, 1>(a, st);
-    if (a.per <= 2) return launch_route_wave<T, SIGMOID, 2>(a, st);
-    if (a.per <= 4) return launch_route_wave<T, SIGMOID, 4>(a, st);
-    if (a.per <= 8) return launch_route_wave<T, SIGMOID, 8>(a, st);
-    if (a.per <= 16) return launch_route_wave<T, SIGMOID, 16>(a, st);
+    // The groups over 64 lanes: a power of two each, 16 at most (what rates them stays inside 16 lanes), and a power of two of experts for every lane; 1024 experts
+    // in up to 64 groups come to 32 at most.
+    a.group_shift = 0;
+    while (a.n_groups << (a.group_shift + 1) <= 64 && (a.group_shift < 4 || a.n_groups == 1)) a.group_shift++;
+    int ne = 1;
+    while (ne << a.group_shift < a.group_size) ne *= 2;
+    // Four tokens a wave where there are waves enough that way (8 of 256 in 8 groups, four against one: 1024 tokens 6.3 and 4.9 us, 4096 6.9 and 7.7, 8192 8.4
+    // and 11.7; 16 of 512, 8192 tokens: 19.1 and 22.8).
+    if (a.n_tokens >= env_int("CAMELID_HIP_ROUTE_QUARTER", 4096) && a.k <= 16 && a.group_shift >= 2 && ne <= 8) {
+        a.group_shift -= 2;
+        return a.k <= 8 ? launch_route_quarters<T, SIGMOID, 8>(a, 4 * ne, st) : launch_route_quarters<T, SIGMOID, 16>(a, 4 * ne, st);
+    }
+    if (ne == 1) return launch_route_wave<T, SIGMOID, 1>(a, st);
+    if (ne == 2) return launch_route_wave<T, SIGMOID, 2>(a, st);
+    if (ne == 4) return launch_route_wave<T, SIGMOID, 4>(a, st);
+    if (ne == 8) return launch_route_wave<T, SIGMOID, 8>(a, st);
+    if (ne == 16) return launch_route_wave<T, SIGMOID, 16>(a, st);
     return launch_route_wave<T, SIGMOID, 32>(a, st);
 }
 
 int launch_moe_route_scored(int score, int dtype, const void *logits, int64_t stride, const float *bias, int64_t n_tokens, int n_experts, int n_groups, int groups_kept, int group_top, int k,
                             int renormalise, float weight_scale, int32_t *idx, float *weight, hipStream_t st) {
     const int size = n_experts / n_groups;
-    const RouteArgs a{logits, bias, idx, weight, stride, n_tokens, n_experts, n_groups, groups_kept, group_top, k, size, 0, 0, renormalise, weight_scale};
+    const RouteArgs a{logits, bias, idx, weight, stride, n_tokens, n_experts, n_groups, groups_kept, group_top, k, size, 0, renormalise, weight_scale};
     return with_type(dtype, [&](auto t) { return score == CML_ROUTE_SIGMOID ? launch_route<decltype(t), true>(a, st) : launch_route<decltype(t), false>(a, st); });
 }
 

@@ -112,6 +112,10 @@ __device__ __forceinline__ int row_allmin_i32(int v) {
     return min(v, row_ror_i32<8>(v));
 }
 __device__ __forceinline__ float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+__device__ __forceinline__ float rows_allsum(float v) {  // rows of 16 like row_allsum, then the four of them
+    v = row_allsum(v);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
 __device__ __forceinline__ float wave_allsum(float v) {
     v = v + dpp_f32<0x121>(v);  // row_ror 1, 2, 4, 8: the sum of the row of 16 in all its lanes (each with its own association: one lane is read)
     v = v + dpp_f32<0x122>(v);

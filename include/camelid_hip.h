@@ -461,7 +461,8 @@ int cml_matmul_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev
  *   the k best keys of the groups that stay, in descending order, ties to the lower index throughout
  *   weight = score, divided by the sum of the chosen scores if renormalise, times weight_scale
  * An expert whose logit or key is -inf or NaN takes no part; slots without an expert have id -1 and weight 0.
- * +inf counts as the largest finite logit.  Up to 1024 experts, 64 groups, k up to 64. */
+ * +inf counts as the largest finite logit.  Up to 1024 experts, 64 groups, k up to 64.  A token's bits do
+ * not depend on n_tokens. */
 enum { CML_ROUTE_SOFTMAX = 0, CML_ROUTE_SIGMOID = 1 };
 int cml_moe_route_scored(int score, int dtype, const void *logits_dev, int64_t logits_stride,
                          const float *bias_dev, int64_t n_tokens, int n_experts, int n_groups,
@@ -470,7 +471,8 @@ int cml_moe_route_scored(int score, int dtype, const void *logits_dev, int64_t l
 /* For every row of logits and its given token target[row]: the token's log probability; its rank (1 = the
  * largest logit; ties count lower indices first; nullable); the row's entropy in nats (nullable); the
  * n_top (0 to 64) best tokens in order, ties to the lower index, with their log probabilities
- * (top_ids int32[n_rows*n_top], top_log_probs f32; null for n_top = 0).  Sums in f32.
+ * (top_ids int32[n_rows*n_top], top_log_probs f32; null for n_top = 0).  Sums in f32, cut by n_rows and
+ * vocab: the last bits may differ between calls of different n_rows, and with them only.
  * -inf is a masked token: probability 0, never an alternative; slots without a token have id -1 and
  * -inf.  A row of masked tokens: log probability -inf, entropy 0.  A target outside the
  * vocabulary: log probability NaN, rank 0.  NaN or +inf in a row: NaN in log probabilities and entropy.

@@ -153,6 +153,19 @@ def test_groups_of_any_size(experts, groups, kept, group_top, k):
     compare(SIGMOID, "f16", logits, (rng.integers(-8, 8, experts) / 64.0).astype(np.float32), groups, kept, group_top, k, pad=1)
 
 
+@pytest.mark.parametrize("experts,groups,kept,group_top,k", [(64, 1, 1, 1, 6), (100, 1, 1, 1, 8), (128, 2, 1, 2, 8), (160, 8, 3, 2, 6), (192, 16, 4, 1, 16), (256, 8, 4, 2, 8), (300, 3, 2, 2, 9), (512, 1, 1, 1, 10)])
+def test_a_token_does_not_depend_on_the_batch(experts, groups, kept, group_top, k):
+    rng = np.random.default_rng(experts)
+    logits = to_bits(2 * rng.standard_normal((40, experts)), "f32")
+    bias = (0.1 * rng.standard_normal(experts)).astype(np.float32)
+    for score in (SOFTMAX, SIGMOID):
+        for b in (None, bias):
+            few = route(score, "f32", logits, b, groups, kept, group_top, k)
+            with G.env(CAMELID_HIP_ROUTE_QUARTER=1), G.engaged("^moe.route.scored.quarter$"):
+                many = route(score, "f32", logits, b, groups, kept, group_top, k)
+            assert np.array_equal(few[0], many[0]) and np.array_equal(few[1].view(np.uint32), many[1].view(np.uint32))
+
+
 @pytest.mark.parametrize("n", [4095, 4096, 4098])
 def test_long_prompts(n):
     rng = np.random.default_rng(n)
