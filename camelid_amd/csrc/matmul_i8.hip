@@ -37,11 +37,17 @@ __device__ __forceinline__ void store_cells(const MatmulI8 &a, int t, int r, con
         }
 }
 
+// A pointer that is the same in all lanes, for an operand that has to be in scalar registers.
+__device__ __forceinline__ const int8_t *wave_uniform(const int8_t *p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)), high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const int8_t *>(static_cast<uint64_t>(high) << 32 | low);
+}
+
 // ---- few tokens -----------------------------------------------------------------------------------------
-// Up to 16 tokens: the weight's bytes are the time.  A workgroup owns 16 weight rows; its waves take the 128-byte lines of the rows in turn, so that all
-// of a short row is requested at once, and their sums meet in LDS.  Operands go from memory to registers: lane 16 k + n holds 16 bytes of row
-// (token) n, and which bytes of the line does not matter as long as both operands agree.  Any alignment, any length.  One token on 4096 x 4096 (17 MB):
-// 5.9 us, on 14336 x 4096 15.0 (3.9 TB/s): a compute unit takes in 40 to 60 GB/s here however much is in flight (eight, twelve and sixteen waves, two to twelve steps ahead).
+// Rows that start anywhere, up to 16 tokens: the weight's bytes are the time.  A workgroup owns 16 weight rows; its waves take the 128-byte lines of the rows in turn, so that
+// all of a short row is requested at once, and their sums meet in LDS.  Operands go from memory to registers: lane 16 k + n holds 16 bytes of row (token) n, and
+// which bytes of the line does not matter as long as both operands agree.  Any alignment, any length.  One token on 14336 x 4096: 15.5 us.
 template <class T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void matmul_i8_few_kernel(MatmulI8 a) {
     constexpr int U = 2;  // lines of every row in one batch of requests
@@ -119,6 +125,106 @@ static int launch_few(const MatmulI8 &a, hipStream_t st) {
     return CML_OK;
 }
 
+// ---- slim tiles -----------------------------------------------------------------------------------------
+// Rows on 16-byte boundaries, and few cells or short time: 16 or 32 weight rows by 16 to 64 tokens a workgroup, so that a product of few cells still has a workgroup for
+// every compute unit, and each of its waves takes lines of the rows in turn, by itself: it has LDS of its own, a ring of STAGES lines that requests fill directly, waits for its own
+// requests only, and meets the others where the sums are added up.  A request brings whole lines, eight to an instruction (what a unit takes in goes by lines in flight; from
+// memory to registers, 16 half lines to an instruction, it was half as much).  Slot p of a row holds piece p ^ key(row), as below.
+//
+// 16 tokens on 4096 x 14336: 13.5 us (through registers 18.5), on 352 x 15040 8.7 (21); 32 tokens on 4096 x 14336 16.6 (in tiles of 64 x 32 31.6), 64 on 1024 x 4096 5.2 (8.8).  What
+// bounds it is the weight's way from memory (4.9 TB/s of it at 4096 x 14336, one token) and for more tokens theirs from the L2.
+template <class T, int RT, int TT, int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) {
+    constexpr int kRows = 16 * RT, kStage = 16 * (RT + TT) * 128, kFetches = 2 * (RT + TT);
+    extern __shared__ uint4 smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, kq = lane >> 4;
+    int row_block, column;
+    const int n_row_blocks = (a.rows + kRows - 1) / kRows, n_columns = (a.n_tokens + 16 * TT - 1) / (16 * TT);
+    if (a.rows >= a.n_tokens ? !wide_block(blockIdx.x, n_row_blocks, n_columns, row_block, column) : !wide_block(blockIdx.x, n_columns, n_row_blocks, column, row_block)) return;
+    const int r0 = row_block * kRows, t0 = column * 16 * TT;
+    const int lines = a.cols >> 7, mine = lines > wave ? (lines - wave + WAVES - 1) / WAVES : 0;
+    const int8_t *w0 = a.w + static_cast<int64_t>(r0) * a.w_stride + wave * 128, *q0 = a.q + t0 * a.q_stride + wave * 128;
+    uint32_t src[kFetches];  // rows 8 f .. 8 f + 7 of the stage: lane 8 r + p brings piece p ^ key(row) of row r
+#pragma unroll
+    for (int f = 0; f < kFetches; f++) {
+        const int at = f * 8 + (lane >> 3);
+        const uint32_t piece = ((lane & 7) ^ (at >> 1 & 7)) << 4;
+        src[f] = f < 2 * RT ? static_cast<uint32_t>(min(at, a.rows - 1 - r0)) * static_cast<uint32_t>(a.w_stride) + piece
+                            : static_cast<uint32_t>(min(at - kRows, a.n_tokens - 1 - t0)) * static_cast<uint32_t>(a.q_stride) + piece;
+    }
+    const int8_t *lds = reinterpret_cast<const int8_t *>(smem) + wave * (STAGES * kStage);
+    const uint32_t lds0 = lds_address(smem) + wave * (STAGES * kStage);
+    auto fetch = [&](int i, int stage) __attribute__((always_inline)) {
+        const int64_t at = static_cast<int64_t>(min(i, mine - 1)) * (WAVES * 128);
+#pragma unroll
+        for (int f = 0; f < kFetches; f++) wide_dma16(lds0 + stage * kStage + f * 1024, wave_uniform((f < 2 * RT ? w0 : q0) + at), src[f]);
+    };
+    v4i_i8 acc[RT][TT] = {};
+    auto multiply = [&](const v4i_i8 (&w)[RT][2], const v4i_i8 (&q)[TT][2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int t = 0; t < TT; t++) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r][h], q[t][h], acc[r][t], 0, 0, 0);
+    };
+    if (mine > 0) {
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; k++) fetch(k, k);
+        int stage = 0, into = STAGES - 1;
+        for (int i = 0; i < mine; i++) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read last may be overwritten
+            fetch(i + STAGES - 1, into);                        // (past the end the last line again: the number of requests in flight stays the same)
+            wide_wait<(STAGES - 1) * kFetches>();
+            v4i_i8 w[RT][2], q[TT][2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int8_t *at = lds + stage * kStage + n * 128 + (((4 * h + kq) ^ (n >> 1)) << 4);
+#pragma unroll
+                for (int r = 0; r < RT; r++) w[r][h] = *reinterpret_cast<const v4i_i8 *>(at + r * 2048);
+#pragma unroll
+                for (int t = 0; t < TT; t++) q[t][h] = *reinterpret_cast<const v4i_i8 *>(at + (RT + t) * 2048);
+            }
+            multiply(w, q);
+            into = stage;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        }
+        wide_wait<0>();
+    }
+    if ((a.cols & 127) && lines % WAVES == wave) {  // the rest of the rows, zeros behind their ends
+        auto piece = [&](const int8_t *p, int c) {
+            v4i_i8 v = {};
+            if (c + 16 <= a.cols) return *reinterpret_cast<const v4i_i8 *>(p + c);
+            for (int j = 0; c + j < a.cols; j++) v[j >> 2] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(p[c + j])) << (8 * (j & 3)));
+            return v;
+        };
+        v4i_i8 w[RT][2], q[TT][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int c = lines * 128 + (4 * h + kq) * 16;
+#pragma unroll
+            for (int r = 0; r < RT; r++) w[r][h] = piece(a.w + static_cast<int64_t>(min(r0 + 16 * r + n, a.rows - 1)) * a.w_stride, c);
+#pragma unroll
+            for (int t = 0; t < TT; t++) q[t][h] = piece(a.q + static_cast<int64_t>(min(t0 + 16 * t + n, a.n_tokens - 1)) * a.q_stride, c);
+        }
+        multiply(w, q);
+    }
+    __syncthreads();  // (LDS changes its use)
+    v4i_i8 *part = reinterpret_cast<v4i_i8 *>(smem);
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int t = 0; t < TT; t++) part[((r * TT + t) * WAVES + wave) * 64 + lane] = acc[r][t];
+    __syncthreads();
+    for (int c = wave; c < RT * TT; c += WAVES) {
+        v4i_i8 sum = {};
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) sum += part[(c * WAVES + k) * 64 + lane];
+        store_cells<T>(a, t0 + 16 * (c % TT) + n, r0 + 16 * (c / TT) + 4 * kq, sum);
+    }
+}
+
 // ---- tiles --------------------------------------------------------------------------------------------
 // Rows on 16-byte boundaries.  WR x WT waves of MT x NT tiles of 32 x 32 cells; a step is 128 values of the contraction: whole lines of both operands
 // go to LDS without passing through registers, into the oldest of STAGES steps as soon as it has been read.  Slot p of an LDS row (16 bytes) holds piece p ^ key(row), so that the eight rows that
@@ -141,13 +247,6 @@ __device__ __forceinline__ void tile_of(const TileGrid &g, int at, int &row_bloc
     wide = min(g.group, g.n_token_blocks - band * g.group);
     row_block = in / wide;
     token_block = band * g.group + in - row_block * wide;
-}
-
-// A pointer that is the same in all lanes, for an operand that has to be in scalar registers.
-__device__ __forceinline__ const int8_t *wave_uniform(const int8_t *p) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)), high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-    return reinterpret_cast<const int8_t *>(static_cast<uint64_t>(high) << 32 | low);
 }
 
 // One tile's work by a workgroup of WR x WT waves.  SPLIT: the tile has 1 / SPLIT of the rows.  FULL: every row and token of the tile is there.
@@ -611,6 +710,19 @@ static int launch_tile(const MatmulI8 &a, hipStream_t st) {
     return CML_OK;
 }
 
+template <class T, int RT, int TT, int WAVES, int STAGES>
+static int launch_slim(const MatmulI8 &a, hipStream_t st) {
+    constexpr int kLds = WAVES * STAGES * 16 * (RT + TT) * 128;
+    static_assert(kLds <= 160 * 1024 && kLds >= RT * TT * WAVES * 1024, "LDS");
+    const int n_row_blocks = (a.rows + 16 * RT - 1) / (16 * RT), n_columns = (a.n_tokens + 16 * TT - 1) / (16 * TT);
+    const auto kernel = matmul_i8_slim_kernel<T, RT, TT, WAVES, STAGES>;
+    static std::atomic<bool> raised{false};
+    if (int rc = allow_lds(kernel, kLds, raised)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(a.rows >= a.n_tokens ? wide_grid(n_row_blocks, n_columns) : wide_grid(n_columns, n_row_blocks)), dim3(64 * WAVES), kLds, st, a);
+    CML_HIP_TRY(hipGetLastError());
+    return CML_OK;
+}
+
 template <class T, int MT>
 static int launch_staged(const MatmulI8 &a, hipStream_t st) {
     typedef TileWork<T, 2, 2, MT, MT, 2, false, false> Work;
@@ -634,24 +746,28 @@ static int launch_walk(const MatmulI8 &a, hipStream_t st) {
     return CML_OK;
 }
 
-// What a call takes by tile, in microseconds: a start of 3, then per workgroup that a compute unit runs `work` for each step of 128 values and `ends` for the tile;
-// no tile is through its steps faster than `step` each, alone on its unit.  Fitted to 1 - 4096 tokens on nine weight shapes (704 x 2816 to 128256 x 2048):
-// the tile that it picks takes 0.8 % more than the best one in the mean, 13 % at most.
+// What a call takes by tile, in microseconds: a start, then per workgroup that a compute unit runs `work` for each step of 128 values and `ends` for the tile;
+// no tile is through its steps faster than `step` each, alone on its unit.  Fitted to 1 - 4096 tokens on weights from 64 x 512 to 128256 x 2048: the tile that it picks takes
+// 0.8 % more than the best one in the mean, 25 % at most.
 struct TileCost {
     int rows, tokens, per_unit;
-    float step, work, ends;
+    float start, step, work, ends;
 };
-constexpr TileCost kWalk{256, 256, 1, 1.12f, 0.85f, 6.2f}, kTiles[] = {{256, 128, 1, 0.73f, 0.63f, 3.2f}, {128, 128, 1, 0.51f, 0.435f, 2.9f}, {64, 128, 2, 0.36f, 0.32f, 0.92f},
-                                                                       {64, 64, 2, 0.236f, 0.213f, 0.5f}, {64, 32, 3, 0.213f, 0.174f, 0.4f}};
+constexpr TileCost kWalk{256, 256, 1, 3.0f, 1.12f, 0.85f, 6.2f},
+    kTiles[] = {{256, 128, 1, 3.0f, 0.73f, 0.63f, 3.2f},   {128, 128, 1, 3.0f, 0.51f, 0.435f, 2.9f},   {64, 128, 2, 3.0f, 0.36f, 0.32f, 0.92f},
+                {64, 64, 2, 3.0f, 0.236f, 0.213f, 0.5f},   {64, 32, 3, 3.0f, 0.213f, 0.174f, 0.4f},    {16, 16, 3, 2.5f, 0.054f, 0.049f, 0.425f},
+                {32, 16, 2, 2.5f, 0.078f, 0.073f, 0.663f}, {16, 32, 3, 2.5f, 0.08f, 0.074f, 0.427f},   {32, 32, 2, 2.5f, 0.117f, 0.104f, 0.662f},
+                {16, 64, 2, 2.5f, 0.136f, 0.124f, 0.755f}, {32, 64, 1, 2.5f, 0.052f, 0.153f, 2.217f}};
 static float tile_cost(const MatmulI8 &a, const TileCost &c) {
     const int64_t tiles = static_cast<int64_t>((a.rows + c.rows - 1) / c.rows) * ((a.n_tokens + c.tokens - 1) / c.tokens);
     const float steps = static_cast<float>((a.cols + 127) / 128), one = c.work * steps + c.ends;
-    if (&c == &kWalk) return 3.0f + std::max(c.step * steps, std::max(1.0f, 0.5f * static_cast<float>((tiles + 127) / 128)) * one);  // (half rounds)
+    if (&c == &kWalk) return c.start + std::max(c.step * steps, std::max(1.0f, 0.5f * static_cast<float>((tiles + 127) / 128)) * one);  // (half rounds)
     const int64_t full = tiles / (256 * c.per_unit), left = tiles - full * 256 * c.per_unit;
-    return 3.0f + static_cast<float>(full * c.per_unit) * one + (left ? std::max(c.step * steps, static_cast<float>((left + 255) / 256) * one) : 0.0f);
+    return c.start + static_cast<float>(full * c.per_unit) * one + (left ? std::max(c.step * steps, static_cast<float>((left + 255) / 256) * one) : 0.0f);
 }
 
-// Variants: 0 the walk, 1 - 5 kTiles, 6 / 7 tiles of 128 x 64 / 64 x 64 that ask for the weight past the caches, 8 / 9 few tokens with eight / four waves.
+// Variants: 0 the walk, 1 - 5 the first of kTiles, 6 / 7 tiles of 128 x 64 / 64 x 64 that ask for the weight past the caches, 8 / 9 few tokens through registers with eight / four
+// waves, 10 - 15 the slim ones.
 static int choose_variant(const MatmulI8 &a) {
     const int64_t bytes = static_cast<int64_t>(a.rows) * a.cols;
     // A weight of 96 MB and more is used once in a pass over a model: past the caches (128256 x 2048, 1 / 16 / 37 tokens: 52 / 55 / 59 us plain, 45 / 46 / 49 so), in the
@@ -660,20 +776,17 @@ static int choose_variant(const MatmulI8 &a) {
         if ((a.rows + 127) / 128 >= 512) return 6;
         if (a.n_tokens <= 32) return 7;
     }
-    int best = 1;
+    int best = 0;
     float least = tile_cost(a, kTiles[0]);
-    for (int i = 1; i < 5; i++) {
+    for (int i = 1; i < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); i++) {
         const float c = tile_cost(a, kTiles[i]);
         if (c < least) {
             least = c;
-            best = i + 1;
+            best = i;
         }
     }
     if (a.rows >= 256 && a.n_tokens >= 256 && tile_cost(a, kWalk) < least) return 0;
-    // Few tokens: no steps to wait for, but every workgroup reads the tokens for itself (4096 x 14336, 1 / 16 tokens: 13.9 / 18.3 us, tiles 30 / 31; 14336 x 4096: 15.0 / 20.0
-    // and 15.3 / 15.8).  Four waves from 8192 rows (8192 x 1024: 4.3 us, eight 4.4; 128256 x 2048: 48 and 61).
-    if (a.n_tokens <= 16 && 3.0f + (0.17f + 0.0055f * static_cast<float>(a.n_tokens)) * 1e-6f * static_cast<float>(bytes) < least) return a.rows < 8192 ? 8 : 9;
-    return best;
+    return best < 5 ? best + 1 : best + 5;
 }
 
 template <class T>
@@ -688,6 +801,12 @@ static int launch_variant(int v, const MatmulI8 &a, hipStream_t st) {
         case 6: return launch_tile<T, 4, 1, 1, 2, 3, 2, true>(a, st);
         case 7: return launch_tile<T, 2, 2, 1, 1, 4, 2, true>(a, st);
         case 8: return launch_few<T, 8>(a, st);
+        case 10: return launch_slim<T, 1, 1, 4, 3>(a, st);
+        case 11: return launch_slim<T, 2, 1, 4, 3>(a, st);
+        case 12: return launch_slim<T, 1, 2, 4, 2>(a, st);
+        case 13: return launch_slim<T, 2, 2, 4, 2>(a, st);
+        case 14: return launch_slim<T, 1, 4, 4, 2>(a, st);
+        case 15: return launch_slim<T, 2, 4, 4, 2>(a, st);
         default: return launch_few<T, 4>(a, st);
     }
 }
@@ -699,14 +818,16 @@ int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int
                          q_stride < (1 << 23) && w_stride < (1 << 23);  // (256 rows within 32 bits)
     const int forced = env_int("CAMELID_HIP_I8_TILE", 0);  // n: variant n - 1 where it serves the call; -1: staged
     int v = choose_variant(a);
-    if (forced > 0 && forced <= 10 && !(forced == 1 && (rows < 256 || n_tokens < 256)) && !(forced >= 9 && n_tokens > 16)) v = forced - 1;
-    if (!aligned && v < 8 && n_tokens <= 16 && forced >= 0) v = rows < 8192 ? 8 : 9;
-    if (forced >= 0 && (aligned || v >= 8)) {
+    if (forced > 0 && forced <= 16 && !(forced == 1 && (rows < 256 || n_tokens < 256)) && !((forced == 9 || forced == 10) && n_tokens > 16)) v = forced - 1;
+    // Through registers: four waves from 8192 rows (one token on 8192 x 1024: 4.3 us, eight 4.4; on 128256 x 2048 48 and 61).
+    if (!aligned && n_tokens <= 16 && v != 8 && v != 9) v = rows < 8192 ? 8 : 9;
+    if (forced >= 0 && (aligned || v == 8 || v == 9)) {
         switch (v) {
             case 0: CML_COUNT_LAUNCH("i8.matmul.walk"); break;
             case 8: case 9: CML_COUNT_LAUNCH("i8.matmul.few"); break;
             case 6: case 7: CML_COUNT_LAUNCH("i8.matmul.tile.once"); break;
-            default: CML_COUNT_LAUNCH("i8.matmul.tile"); break;
+            case 1: case 2: case 3: case 4: case 5: CML_COUNT_LAUNCH("i8.matmul.tile"); break;
+            default: CML_COUNT_LAUNCH("i8.matmul.slim"); break;
         }
         return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
     }

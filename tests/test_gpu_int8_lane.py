@@ -165,21 +165,22 @@ def test_product_strides_alignments_and_no_bias(t, n, rows, cols, q_pad, w_pad, 
 
 
 # every kernel that can serve a call gives the same bits: whole and cut tiles, one step and many, rows that end inside a step and inside 16 bytes
-@pytest.mark.parametrize("n,rows,cols", [(256, 256, 64), (300, 700, 128), (257, 2400, 272), (640, 5000, 400), (2500, 2300, 130), (16, 300, 1100), (2, 5000, 127), (1030, 4100, 512)])
+@pytest.mark.parametrize("n,rows,cols", [(256, 256, 64), (300, 700, 128), (257, 2400, 272), (640, 5000, 400), (2500, 2300, 130), (16, 300, 1100), (2, 5000, 127), (1030, 4100, 512), (1, 17, 5000), (33, 100, 128), (70, 33, 2057)])
 def test_product_by_every_kernel(n, rows, cols):
     q, w, s, ws, bias = operands(n * rows, n, rows, cols)
     pad = -cols % 16
     t = ["f32", "f16", "bf16"][rows % 3]
     want = want_product(t, q, w, s, ws, bias)
-    for tile, kernel in [(-1, "staged"), (1, "walk"), (2, "tile"), (3, "tile"), (4, "tile"), (5, "tile"), (6, "tile"), (7, "tile.once"), (8, "tile.once"), (9, "few"), (10, "few")]:
-        if (tile == 1 and n < 256) or (tile >= 9 and n > 16):
+    for tile, kernel in [(-1, "staged"), (1, "walk"), (2, "tile"), (3, "tile"), (4, "tile"), (5, "tile"), (6, "tile"), (7, "tile.once"), (8, "tile.once"), (9, "few"), (10, "few"),
+                         (11, "slim"), (12, "slim"), (13, "slim"), (14, "slim"), (15, "slim"), (16, "slim")]:
+        if (tile == 1 and n < 256) or (tile in (9, 10) and n > 16):
             continue
         with G.env(CAMELID_HIP_I8_TILE=tile), G.engaged(f"^i8.matmul.{kernel}$"):
             assert np.array_equal(product(t, q, w, s, ws, bias, q_pad=pad, w_pad=pad), want), tile
 
 
 def test_kernels_by_size():
-    for n, rows, cols, pad, kernel in [(1, 512, 1024, 0, "few"), (1, 512, 1024, 1, "few"), (40, 512, 1024, 0, "tile"), (40, 512, 1024, 1, "staged"), (40, 98304, 1024, 0, "tile.once"), (2048, 8192, 512, 0, "walk")]:
+    for n, rows, cols, pad, kernel in [(1, 512, 1024, 0, "slim"), (1, 512, 1024, 1, "few"), (40, 512, 1024, 0, "slim"), (400, 4096, 512, 0, "tile"), (40, 512, 1024, 1, "staged"), (40, 98304, 1024, 0, "tile.once"), (2048, 8192, 512, 0, "walk")]:
         q, w, s, ws, _ = operands(n, n, rows, cols)
         with G.engaged(f"^i8.matmul.{kernel}$"):
             assert np.array_equal(product("f32", q, w, s, ws, None, q_pad=pad, w_pad=pad), want_product("f32", q, w, s, ws, None))
