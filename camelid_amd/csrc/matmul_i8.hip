@@ -232,8 +232,8 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) 
 //
 // The instruction's 32 rows are the tile's in another order: a lane ends up with 16 neighbouring weight rows of its token and stores them whole.
 //
-// 37 tokens on 128256 x 2048: 50 us, the weight and the logits at 5.6 TB/s.  4096 x 14336 x 4096 (the walk): 241 us, 2.0 POPS; the matrix cores execute 54 % of the busy
-// cycles, LDS conflicts are gone, and the clock is the limit: under this load it falls from 2.4 to 1.8 GHz (8192 x 8192 x 8192: 459 us, of zeros 335).
+// 37 tokens on 128256 x 2048: 50 us, the weight and the logits at 5.6 TB/s.  4096 x 14336 x 4096 (the walk): 222 us, 2.2 POPS; the matrix cores execute 54 % of the busy
+// cycles, LDS conflicts are gone, and the clock is the limit: under this load it falls from 2.4 to 1.8 GHz (8192 x 8192 x 8192: 451 us, of zeros 335).
 typedef int v16i_i8 __attribute__((ext_vector_type(16)));
 
 struct TileGrid {
@@ -474,7 +474,8 @@ struct TileWork {
     }
     // A lane has 16 neighbouring rows of one token: stored so, a wave would write 16 bytes here and there (256 x 256 cells 10 us).  They change places in LDS, each
     // wave's in its own 8 KB of the second stage, 32 tokens by up to 256 bytes at a time, and leave as whole runs.  Slots are exclusive-ored here too.
-    template <int SPLIT>
+    // STREAM: past the caches.
+    template <int SPLIT, bool STREAM = false>
     __device__ __forceinline__ void store(uint4 *smem, int row, int token) {
         row = __builtin_amdgcn_readfirstlane(row);
         token = __builtin_amdgcn_readfirstlane(token);
@@ -542,7 +543,8 @@ struct TileWork {
                     Bits *out = static_cast<Bits *>(a.out) + (t0 + t) * a.out_stride + rr;
                     if (FULL || rr + kPer <= a.rows) {
                         typedef uint32_t v4u __attribute__((ext_vector_type(4), aligned(2)));
-                        *reinterpret_cast<v4u *>(out) = v4u{v.x, v.y, v.z, v.w};
+                        if constexpr (STREAM) __builtin_nontemporal_store(v4u{v.x, v.y, v.z, v.w}, reinterpret_cast<v4u *>(out));
+                        else *reinterpret_cast<v4u *>(out) = v4u{v.x, v.y, v.z, v.w};
                     } else {
                         const uint32_t word[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -644,7 +646,7 @@ __global__ __launch_bounds__(256) void matmul_i8_staged_kernel(MatmulI8 a, TileG
 // it has.  The tiles that are left when all 32 can no longer have a whole one are cut into halves or quarters of their rows where that gives every
 // unit some (896 tiles, 4096 tokens on 14336 rows: the time of 3.5 tiles instead of 4).  The last tiles of a side that is no whole number of them reach back
 // into their neighbours: cells that two workgroups write get the same bits.
-template <class T, int WR, int WT, int MT, int NT>
+template <class T, int WR, int WT, int MT, int NT, bool STREAM>
 __global__ __launch_bounds__(64 * WR * WT, WR * WT / 4) void matmul_i8_walk_kernel(MatmulI8 a, TileGrid grid) {
     extern __shared__ uint4 smem[];
     TileWork<T, WR, WT, MT, NT, 2, false, true> work(a, smem);
@@ -687,7 +689,7 @@ __global__ __launch_bounds__(64 * WR * WT, WR * WT / 4) void matmul_i8_walk_kern
             constexpr int kParts = decltype(parts)::value;
             work.template sums<kParts>(smem);
             if (item + 1 < items) begin(item + 1);
-            work.template store<kParts>(smem, r, t);
+            work.template store<kParts, STREAM>(smem, r, t);
         };
         if (cut == 1) run(std::integral_constant<int, 1>{});
         else if (cut == 2) run(std::integral_constant<int, 2>{});
@@ -747,15 +749,24 @@ static int launch_staged(const MatmulI8 &a, hipStream_t st) {
     return CML_OK;
 }
 
-template <class T>
-static int launch_walk(const MatmulI8 &a, hipStream_t st) {
+template <class T, bool STREAM>
+static int launch_walk_stores(const MatmulI8 &a, hipStream_t st) {
     typedef TileWork<T, 2, 4, 4, 2, 2, false, true> Work;
-    const auto kernel = matmul_i8_walk_kernel<T, 2, 4, 4, 2>;
+    const auto kernel = matmul_i8_walk_kernel<T, 2, 4, 4, 2, STREAM>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
     hipLaunchKernelGGL(kernel, dim3(256), dim3(Work::kThreads), Work::kLds, st, a, tile_grid(a, Work::kRows, Work::kTokens));
     CML_HIP_TRY(hipGetLastError());
     return CML_OK;
+}
+template <class T>
+static int launch_walk(const MatmulI8 &a, hipStream_t st) {
+    // An output of 96 MB and more, in whole lines, leaves past the caches, which do not hold it for the next kernel anyway (4096 tokens on 14336 x 4096, bf16, 117 MB: 242 us plain, 219
+    // so, with a copy of it behind 284 and 280).  For smaller ones the next kernel pays (1024 tokens on 4096 x 4096: 24.0 and 21.6, with the copy 27.3 and 27.9), for rows that start
+    // inside a line this one does (3461 tokens on 59669 x 128: 152 and 232).
+    constexpr int kSize = sizeof(typename T::Bits);
+    const bool lines = ((reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.out_stride * kSize)) & 127u) == 0;
+    return lines && static_cast<int64_t>(a.n_tokens) * a.rows * kSize >= 96ll << 20 ? launch_walk_stores<T, true>(a, st) : launch_walk_stores<T, false>(a, st);
 }
 
 // What a call takes by tile, in microseconds: a start, then per workgroup that a compute unit runs `work` for each step of 128 values and `ends` for the tile;

@@ -186,6 +186,23 @@ def test_kernels_by_size():
             assert np.array_equal(product("f32", q, w, s, ws, None, q_pad=pad, w_pad=pad), want_product("f32", q, w, s, ws, None))
 
 
+@pytest.mark.parametrize("t,n,rows,out_pad", [("bf16", 3100, 16512, 0), ("bf16", 3100, 16513, 0), ("f32", 1700, 16384, 32), ("f32", 1700, 16384, 1)])
+def test_large_outputs(t, n, rows, out_pad):
+    """On either side of whole lines; columns at random against the formula, all of them against the sum over rows."""
+    cols = 144
+    q, w, s, ws, bias = operands(n, n, rows, cols)
+    with G.engaged("^i8.matmul.walk$"):
+        got = product(t, q, w, s, ws, bias, out_pad=out_pad)
+    pick = np.unique(np.concatenate([np.random.default_rng(1).integers(rows, size=600), [0, 255, 256, rows - 257, rows - 1]]))
+    assert np.array_equal(got[:, pick], want_product(t, q, w[pick], s, ws[pick], bias[pick]))
+    total = (q.astype(np.int64) @ w.astype(np.int64).sum(axis=0)).astype(np.float64)
+    exact = (from_bits(got, t).astype(np.float64) - bias.astype(np.float64)) / (s.astype(np.float64)[:, None] * ws.astype(np.float64))
+    # every cell is off by its roundings alone: 2^-7 of itself at most and of the bias, in a sum of signs at random; a cell that was not written would be off by its whole value
+    size = np.abs(from_bits(got, t).astype(np.float64)) + np.abs(bias)
+    bound = (size * 2.0 ** -7 / (s.astype(np.float64)[:, None] * ws.astype(np.float64))).sum(axis=1)
+    assert np.all(np.abs(exact.sum(axis=1) - total) <= bound)
+
+
 @pytest.mark.parametrize("n", [1, 20, 300])
 def test_product_extremes_stay_exact(n):
     cols, rows = 131071 // 16 * 16, 33
