@@ -44,96 +44,18 @@ __device__ __forceinline__ const int8_t *wave_uniform(const int8_t *p) {
     return reinterpret_cast<const int8_t *>(static_cast<uint64_t>(high) << 32 | low);
 }
 
-// ---- few tokens -----------------------------------------------------------------------------------------
-// Rows that start anywhere, up to 16 tokens: the weight's bytes are the time.  A workgroup owns 16 weight rows; its waves take the 128-byte lines of the rows in turn, so that
-// all of a short row is requested at once, and their sums meet in LDS.  Operands go from memory to registers: lane 16 k + n holds 16 bytes of row (token) n, and
-// which bytes of the line does not matter as long as both operands agree.  Any alignment, any length.  One token on 14336 x 4096: 15.5 us.
-template <class T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void matmul_i8_few_kernel(MatmulI8 a) {
-    constexpr int U = 2;  // lines of every row in one batch of requests
-    __shared__ v4i_i8 part[WAVES - 1][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 15, kq = lane >> 4;
-    const int r0 = blockIdx.x * 16;
-    typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
-    const int8_t *w = a.w + min(r0 + n, a.rows - 1) * a.w_stride + 32 * kq, *q = a.q + min(n, a.n_tokens - 1) * a.q_stride + 32 * kq;
-    v4i_i8 acc = {};
-    const int lines = a.cols >> 7;
-    struct Line {
-        v4i_i8 w[2], q[2];
-    };
-    auto load = [&](int line, Line &l) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            l.w[h] = __builtin_nontemporal_load(reinterpret_cast<const v4i_any *>(w + line * 128 + 16 * h));
-            l.q[h] = *reinterpret_cast<const v4i_any *>(q + line * 128 + 16 * h);
-        }
-    };
-    auto multiply = [&](const Line &l) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(l.w[h], l.q[h], acc, 0, 0, 0);
-    };
-    int line = wave;
-    Line now[U], next[U];
-    constexpr int kBatch = U * WAVES, kLast = (U - 1) * WAVES;
-    if (line + kLast < lines) {  // whole batches, the next one requested while this one is multiplied
-#pragma unroll
-        for (int u = 0; u < U; u++) load(line + u * WAVES, now[u]);
-        for (; line + kBatch + kLast < lines; line += kBatch) {
-#pragma unroll
-            for (int u = 0; u < U; u++) load(line + kBatch + u * WAVES, next[u]);
-#pragma unroll
-            for (int u = 0; u < U; u++) multiply(now[u]);
-#pragma unroll
-            for (int u = 0; u < U; u++) now[u] = next[u];
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) multiply(now[u]);
-        line += kBatch;
-    }
-    for (; line < lines; line += WAVES) {
-        load(line, now[0]);
-        multiply(now[0]);
-    }
-    if ((a.cols & 127) && lines % WAVES == wave) {  // the rest of the rows, zeros behind their ends
-        auto piece = [&](const int8_t *p, int c) {
-            if (c + 16 <= a.cols) return static_cast<v4i_i8>(*reinterpret_cast<const v4i_any *>(p));
-            v4i_i8 v = {};
-            for (int j = 0; c + j < a.cols; j++) v[j >> 2] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * (j & 3)));
-            return v;
-        };
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int c = lines * 128 + 32 * kq + 16 * h;
-            now[0].w[h] = piece(w + lines * 128 + 16 * h, c);
-            now[0].q[h] = piece(q + lines * 128 + 16 * h, c);
-        }
-        multiply(now[0]);
-    }
-    if (wave > 0) part[wave - 1][lane] = acc;
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int k = 0; k < WAVES - 1; k++) acc += part[k][lane];
-    store_cells<T>(a, n, r0 + 4 * kq, acc);
-}
-
-template <class T, int WAVES>
-static int launch_few(const MatmulI8 &a, hipStream_t st) {
-    hipLaunchKernelGGL((matmul_i8_few_kernel<T, WAVES>), dim3(static_cast<unsigned>((a.rows + 15) / 16)), dim3(64 * WAVES), 0, st, a);
-    CML_HIP_TRY(hipGetLastError());
-    return CML_OK;
-}
-
 // ---- slim tiles -----------------------------------------------------------------------------------------
-// Rows on 16-byte boundaries, and few cells or short time: 16 or 32 weight rows by 16 to 64 tokens a workgroup, so that a product of few cells still has a workgroup for
-// every compute unit, and each of its waves takes lines of the rows in turn, by itself: it has LDS of its own, a ring of STAGES lines that requests fill directly, waits for its own
-// requests only, and meets the others where the sums are added up.  A request brings whole lines, eight to an instruction (what a unit takes in goes by lines in flight; from
-// memory to registers, 16 half lines to an instruction, it was half as much).  Slot p of a row holds piece p ^ key(row), as below.
+// For few cells: 16 or 32 weight rows by 16 to 64 tokens a workgroup, so that a product of few cells still has a workgroup for every compute unit, and each of its waves takes lines
+// of the rows in turn, by itself: it has LDS of its own, a ring of STAGES lines that requests fill directly, waits for its own requests only, and meets the others where the sums
+// are added up.  A request brings whole lines, eight to an instruction: what a unit takes in goes by the lines it has in flight, and in half lines, sixteen to an instruction, straight to
+// the lanes that multiply them, it is half as much.  Slot p of a row holds piece p ^ key(row), as below.
 //
-// 16 tokens on 4096 x 14336: 13.5 us (through registers 18.5), on 352 x 15040 8.7 (21); 32 tokens on 4096 x 14336 16.6 (in tiles of 64 x 32 31.6), 64 on 1024 x 4096 5.2 (8.8).  What
+// 16 tokens on 4096 x 14336: 13.5 us (in half lines 18.5), on 352 x 15040 8.7 (21); 32 tokens on 4096 x 14336 16.6 (in tiles of 64 x 32 31.6), 64 on 1024 x 4096 4.8 (8.8).  What
 // bounds it is the weight's way from memory (4.9 TB/s of it at 4096 x 14336, one token) and for more tokens theirs from the L2.
-template <class T, int RT, int TT, int WAVES, int STAGES>
+//
+// ANY: rows that start anywhere.  Their lines pass through registers (which takes any address), two of them on their way.  Rows of 4099: one token on 4096 x 4099 5.8 us, 16 6.9;
+// in half lines 8.8 and 13.6.
+template <class T, int RT, int TT, int WAVES, int STAGES, bool ANY>
 __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) {
     constexpr int kRows = 16 * RT, kStage = 16 * (RT + TT) * 128, kFetches = 2 * (RT + TT);
     extern __shared__ uint4 smem[];
@@ -153,13 +75,8 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) 
         src[f] = f < 2 * RT ? static_cast<uint32_t>(min(at, a.rows - 1 - r0)) * static_cast<uint32_t>(a.w_stride) + piece
                             : static_cast<uint32_t>(min(at - kRows, a.n_tokens - 1 - t0)) * static_cast<uint32_t>(a.q_stride) + piece;
     }
-    const int8_t *lds = reinterpret_cast<const int8_t *>(smem) + wave * (STAGES * kStage);
-    const uint32_t lds0 = lds_address(smem) + wave * (STAGES * kStage);
-    auto fetch = [&](int i, int stage) __attribute__((always_inline)) {
-        const int64_t at = static_cast<int64_t>(min(i, mine - 1)) * (WAVES * 128);
-#pragma unroll
-        for (int f = 0; f < kFetches; f++) wide_dma16(lds0 + stage * kStage + f * 1024, wave_uniform((f < 2 * RT ? w0 : q0) + at), src[f]);
-    };
+    typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+    int8_t *lds = reinterpret_cast<int8_t *>(smem) + wave * (STAGES * kStage);
     v4i_i8 acc[RT][TT] = {};
     auto multiply = [&](const v4i_i8 (&w)[RT][2], const v4i_i8 (&q)[TT][2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -169,33 +86,68 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) 
 #pragma unroll
                 for (int t = 0; t < TT; t++) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[r][h], q[t][h], acc[r][t], 0, 0, 0);
     };
-    if (mine > 0) {
+    auto multiply_line = [&](int stage) __attribute__((always_inline)) {
+        v4i_i8 w[RT][2], q[TT][2];
 #pragma unroll
-        for (int k = 0; k < STAGES - 1; k++) fetch(k, k);
-        int stage = 0, into = STAGES - 1;
-        for (int i = 0; i < mine; i++) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read last may be overwritten
-            fetch(i + STAGES - 1, into);                        // (past the end the last line again: the number of requests in flight stays the same)
-            wide_wait<(STAGES - 1) * kFetches>();
-            v4i_i8 w[RT][2], q[TT][2];
+        for (int h = 0; h < 2; h++) {
+            const int8_t *at = lds + stage * kStage + n * 128 + (((4 * h + kq) ^ (n >> 1)) << 4);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int8_t *at = lds + stage * kStage + n * 128 + (((4 * h + kq) ^ (n >> 1)) << 4);
+            for (int r = 0; r < RT; r++) w[r][h] = *reinterpret_cast<const v4i_i8 *>(at + r * 2048);
 #pragma unroll
-                for (int r = 0; r < RT; r++) w[r][h] = *reinterpret_cast<const v4i_i8 *>(at + r * 2048);
-#pragma unroll
-                for (int t = 0; t < TT; t++) q[t][h] = *reinterpret_cast<const v4i_i8 *>(at + (RT + t) * 2048);
-            }
-            multiply(w, q);
-            into = stage;
-            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            for (int t = 0; t < TT; t++) q[t][h] = *reinterpret_cast<const v4i_i8 *>(at + (RT + t) * 2048);
         }
-        wide_wait<0>();
+        multiply(w, q);
+    };
+    if (mine > 0) {
+        if constexpr (ANY) {
+            // lines pass through registers, two of them on their way
+            v4i_i8 one[kFetches], two[kFetches];
+            auto load = [&](v4i_i8 (&to)[kFetches], int i) __attribute__((always_inline)) {
+                const int64_t at = static_cast<int64_t>(min(i, mine - 1)) * (WAVES * 128);
+#pragma unroll
+                for (int f = 0; f < kFetches; f++) to[f] = *reinterpret_cast<const v4i_any *>((f < 2 * RT ? w0 : q0) + at + src[f]);
+            };
+            auto line = [&](v4i_i8 (&of)[kFetches], int i) __attribute__((always_inline)) {
+#pragma unroll
+                for (int f = 0; f < kFetches; f++) *reinterpret_cast<v4i_i8 *>(lds + f * 1024 + lane * 16) = of[f];
+                load(of, i + 2);
+                __builtin_amdgcn_wave_barrier();
+                multiply_line(0);
+                __builtin_amdgcn_wave_barrier();
+            };
+            load(one, 0);
+            load(two, 1);
+            int i = 0;
+            for (; i + 1 < mine; i += 2) {
+                line(one, i);
+                line(two, i + 1);
+            }
+            if (i < mine) line(one, i);
+        } else {
+            const uint32_t lds0 = lds_address(smem) + wave * (STAGES * kStage);
+            auto fetch = [&](int i, int stage) __attribute__((always_inline)) {
+                const int64_t at = static_cast<int64_t>(min(i, mine - 1)) * (WAVES * 128);
+#pragma unroll
+                for (int f = 0; f < kFetches; f++) wide_dma16(lds0 + stage * kStage + f * 1024, wave_uniform((f < 2 * RT ? w0 : q0) + at), src[f]);
+            };
+#pragma unroll
+            for (int k = 0; k < STAGES - 1; k++) fetch(k, k);
+            int stage = 0, into = STAGES - 1;
+            for (int i = 0; i < mine; i++) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read last may be overwritten
+                fetch(i + STAGES - 1, into);                        // (past the end the last line again: the number of requests in flight stays the same)
+                wide_wait<(STAGES - 1) * kFetches>();
+                multiply_line(stage);
+                into = stage;
+                stage = stage == STAGES - 1 ? 0 : stage + 1;
+            }
+            wide_wait<0>();
+        }
     }
     if ((a.cols & 127) && lines % WAVES == wave) {  // the rest of the rows, zeros behind their ends
         auto piece = [&](const int8_t *p, int c) {
             v4i_i8 v = {};
-            if (c + 16 <= a.cols) return *reinterpret_cast<const v4i_i8 *>(p + c);
+            if (c + 16 <= a.cols) return static_cast<v4i_i8>(*reinterpret_cast<const v4i_any *>(p + c));
             for (int j = 0; c + j < a.cols; j++) v[j >> 2] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(p[c + j])) << (8 * (j & 3)));
             return v;
         };
@@ -724,12 +676,12 @@ static int launch_tile(const MatmulI8 &a, hipStream_t st) {
     return CML_OK;
 }
 
-template <class T, int RT, int TT, int WAVES, int STAGES>
+template <class T, int RT, int TT, int WAVES, int STAGES, bool ANY>
 static int launch_slim(const MatmulI8 &a, hipStream_t st) {
     constexpr int kLds = WAVES * STAGES * 16 * (RT + TT) * 128;
     static_assert(kLds <= 160 * 1024 && kLds >= RT * TT * WAVES * 1024, "LDS");
     const int n_row_blocks = (a.rows + 16 * RT - 1) / (16 * RT), n_columns = (a.n_tokens + 16 * TT - 1) / (16 * TT);
-    const auto kernel = matmul_i8_slim_kernel<T, RT, TT, WAVES, STAGES>;
+    const auto kernel = matmul_i8_slim_kernel<T, RT, TT, WAVES, STAGES, ANY>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, kLds, raised)) return rc;
     hipLaunchKernelGGL(kernel, dim3(a.rows >= a.n_tokens ? wide_grid(n_row_blocks, n_columns) : wide_grid(n_columns, n_row_blocks)), dim3(64 * WAVES), kLds, st, a);
@@ -781,6 +733,9 @@ constexpr TileCost kWalk{256, 256, 1, 3.0f, 1.12f, 0.85f, 6.2f},
                 {64, 64, 2, 3.0f, 0.236f, 0.213f, 0.5f},   {64, 32, 3, 3.0f, 0.213f, 0.174f, 0.4f},    {16, 16, 3, 2.5f, 0.054f, 0.049f, 0.425f},
                 {32, 16, 2, 2.5f, 0.078f, 0.073f, 0.663f}, {16, 32, 3, 2.5f, 0.08f, 0.074f, 0.427f},   {32, 32, 2, 2.5f, 0.117f, 0.104f, 0.662f},
                 {16, 64, 2, 2.5f, 0.136f, 0.124f, 0.755f}, {32, 64, 1, 2.5f, 0.052f, 0.153f, 2.217f}};
+// The same for rows that start anywhere: two staged tiles, three slim ones.  Fitted to 1 - 3300 tokens on sixteen weight shapes: 0.3 % more than the best in the mean, 39 % at most.
+constexpr TileCost kAnyTiles[] = {{128, 128, 1, 3.0f, 0.56f, 0.987f, 2.262f}, {64, 64, 2, 3.0f, 0.51f, 0.464f, 0.117f}, {16, 16, 3, 2.5f, 0.033f, 0.105f, 0.348f},
+                                  {32, 16, 2, 2.5f, 0.063f, 0.168f, 0.506f},  {32, 32, 1, 2.5f, 0.163f, 0.227f, 0.764f}};
 static float tile_cost(const MatmulI8 &a, const TileCost &c) {
     const int64_t tiles = static_cast<int64_t>((a.rows + c.rows - 1) / c.rows) * ((a.n_tokens + c.tokens - 1) / c.tokens);
     const float steps = static_cast<float>((a.cols + 127) / 128), one = c.work * steps + c.ends;
@@ -789,9 +744,21 @@ static float tile_cost(const MatmulI8 &a, const TileCost &c) {
     return c.start + static_cast<float>(full * c.per_unit) * one + (left ? std::max(c.step * steps, static_cast<float>((left + 255) / 256) * one) : 0.0f);
 }
 
-// Variants: 0 the walk, 1 - 5 the first of kTiles, 6 / 7 tiles of 128 x 64 / 64 x 64 that ask for the weight past the caches, 8 / 9 few tokens through registers with eight / four
-// waves, 10 - 15 the slim ones.
-static int choose_variant(const MatmulI8 &a) {
+// Variants: 0 the walk, 1 - 5 the first of kTiles, 6 / 7 tiles of 128 x 64 / 64 x 64 that ask for the weight past the caches, 8 - 13 the slim ones; 14 - 18 kAnyTiles.
+template <int N>
+static int cheapest(const MatmulI8 &a, const TileCost (&tiles)[N], float &least) {
+    int best = 0;
+    least = tile_cost(a, tiles[0]);
+    for (int i = 1; i < N; i++) {
+        const float c = tile_cost(a, tiles[i]);
+        if (c < least) {
+            least = c;
+            best = i;
+        }
+    }
+    return best;
+}
+static int choose_aligned(const MatmulI8 &a) {
     const int64_t bytes = static_cast<int64_t>(a.rows) * a.cols;
     // A weight of 96 MB and more is used once in a pass over a model: past the caches (128256 x 2048, 1 / 16 / 37 tokens: 52 / 55 / 59 us plain, 45 / 46 / 49 so), in the
     // tile that has two workgroups for every compute unit (32000 x 4096, 1 / 32 tokens: 128 x 64 31 / 29, 64 x 64 29 / 28; 48 tokens: 30 / 30, plain 24).
@@ -799,17 +766,15 @@ static int choose_variant(const MatmulI8 &a) {
         if ((a.rows + 127) / 128 >= 512) return 6;
         if (a.n_tokens <= 32) return 7;
     }
-    int best = 0;
-    float least = tile_cost(a, kTiles[0]);
-    for (int i = 1; i < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); i++) {
-        const float c = tile_cost(a, kTiles[i]);
-        if (c < least) {
-            least = c;
-            best = i;
-        }
-    }
+    float least;
+    const int best = cheapest(a, kTiles, least);
     if (a.rows >= 256 && a.n_tokens >= 256 && tile_cost(a, kWalk) < least) return 0;
-    return best < 5 ? best + 1 : best + 5;
+    return best < 5 ? best + 1 : best + 3;
+}
+// Rows that start anywhere.
+static int choose_any(const MatmulI8 &a) {
+    float least;
+    return 14 + cheapest(a, kAnyTiles, least);
 }
 
 template <class T>
@@ -823,14 +788,17 @@ static int launch_variant(int v, const MatmulI8 &a, hipStream_t st) {
         case 5: return launch_tile<T, 2, 1, 1, 1, 4, 3>(a, st);
         case 6: return launch_tile<T, 4, 1, 1, 2, 3, 2, true>(a, st);
         case 7: return launch_tile<T, 2, 2, 1, 1, 4, 2, true>(a, st);
-        case 8: return launch_few<T, 8>(a, st);
-        case 10: return launch_slim<T, 1, 1, 4, 3>(a, st);
-        case 11: return launch_slim<T, 2, 1, 4, 3>(a, st);
-        case 12: return launch_slim<T, 1, 2, 4, 2>(a, st);
-        case 13: return launch_slim<T, 2, 2, 4, 2>(a, st);
-        case 14: return launch_slim<T, 1, 4, 4, 2>(a, st);
-        case 15: return launch_slim<T, 2, 4, 4, 2>(a, st);
-        default: return launch_few<T, 4>(a, st);
+        case 8: return launch_slim<T, 1, 1, 4, 3, false>(a, st);
+        case 9: return launch_slim<T, 2, 1, 4, 3, false>(a, st);
+        case 10: return launch_slim<T, 1, 2, 4, 2, false>(a, st);
+        case 11: return launch_slim<T, 2, 2, 4, 2, false>(a, st);
+        case 12: return launch_slim<T, 1, 4, 4, 2, false>(a, st);
+        case 13: return launch_slim<T, 2, 4, 4, 2, false>(a, st);
+        case 14: return launch_staged<T, 2>(a, st);
+        case 15: return launch_staged<T, 1>(a, st);
+        case 16: return launch_slim<T, 1, 1, 4, 1, true>(a, st);
+        case 17: return launch_slim<T, 2, 1, 4, 1, true>(a, st);
+        default: return launch_slim<T, 2, 2, 4, 1, true>(a, st);
     }
 }
 
@@ -839,27 +807,17 @@ int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int
     const MatmulI8 a{q, w, scales, w_scales, bias, out, q_stride, w_stride, out_stride, static_cast<int>(n_tokens), static_cast<int>(rows), static_cast<int>(cols)};
     const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(w) | static_cast<uintptr_t>(q_stride | w_stride)) & 15u) == 0 &&
                          q_stride < (1 << 23) && w_stride < (1 << 23);  // (256 rows within 32 bits)
-    const int forced = env_int("CAMELID_HIP_I8_TILE", 0);  // n: variant n - 1 where it serves the call; -1: staged
-    int v = choose_variant(a);
-    if (forced > 0 && forced <= 16 && !(forced == 1 && (rows < 256 || n_tokens < 256)) && !((forced == 9 || forced == 10) && n_tokens > 16)) v = forced - 1;
-    // Through registers: four waves from 8192 rows (one token on 8192 x 1024: 4.3 us, eight 4.4; on 128256 x 2048 48 and 61).
-    if (!aligned && n_tokens <= 16 && v != 8 && v != 9) v = rows < 8192 ? 8 : 9;
-    if (forced >= 0 && (aligned || v == 8 || v == 9)) {
-        switch (v) {
-            case 0: CML_COUNT_LAUNCH("i8.matmul.walk"); break;
-            case 8: case 9: CML_COUNT_LAUNCH("i8.matmul.few"); break;
-            case 6: case 7: CML_COUNT_LAUNCH("i8.matmul.tile.once"); break;
-            case 1: case 2: case 3: case 4: case 5: CML_COUNT_LAUNCH("i8.matmul.tile"); break;
-            default: CML_COUNT_LAUNCH("i8.matmul.slim"); break;
-        }
-        return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
-    }
-    CML_COUNT_LAUNCH("i8.matmul.staged");
-    // A step takes a compute unit 0.95 us in the tile of 128 x 128, in those of 64 x 64 0.87 two at a time and 0.48 one alone (rows of 4099, 512 x 4096: 37 and 31 us;
-    // 640 x 4096: 38 and 43; 2048 x 2048: 38 and 55).
-    const int64_t four = (rows + 127) / 128 * ((n_tokens + 127) / 128), one = (rows + 63) / 64 * ((n_tokens + 63) / 64), left = one % 512;
-    const bool large = 0.95f * static_cast<float>((four + 255) / 256) < 0.87f * static_cast<float>(one / 512) + (left > 256 ? 0.87f : left > 0 ? 0.48f : 0.0f);
-    return with_type(dtype, [&](auto t) { return large ? launch_staged<decltype(t), 2>(a, st) : launch_staged<decltype(t), 1>(a, st); });
+    const int forced = env_int("CAMELID_HIP_I8_TILE", 0) - 1;  // a variant, where it serves the call
+    const bool near = q_stride < (1 << 26) && w_stride < (1 << 26);  // (64 rows within 32 bits)
+    int v = aligned ? choose_aligned(a) : near ? choose_any(a) : 15;
+    if (near && forced >= (aligned ? 0 : 14) && forced <= 18 && !(forced == 0 && (rows < 256 || n_tokens < 256))) v = forced;
+    if (v == 0) CML_COUNT_LAUNCH("i8.matmul.walk");
+    else if (v < 6) CML_COUNT_LAUNCH("i8.matmul.tile");
+    else if (v < 8) CML_COUNT_LAUNCH("i8.matmul.tile.once");
+    else if (v < 14) CML_COUNT_LAUNCH("i8.matmul.slim");
+    else if (v < 16) CML_COUNT_LAUNCH("i8.matmul.staged");
+    else CML_COUNT_LAUNCH("i8.matmul.slim.any");
+    return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
 }
 
 }  // namespace cml

@@ -171,16 +171,42 @@ def test_product_by_every_kernel(n, rows, cols):
     pad = -cols % 16
     t = ["f32", "f16", "bf16"][rows % 3]
     want = want_product(t, q, w, s, ws, bias)
-    for tile, kernel in [(-1, "staged"), (1, "walk"), (2, "tile"), (3, "tile"), (4, "tile"), (5, "tile"), (6, "tile"), (7, "tile.once"), (8, "tile.once"), (9, "few"), (10, "few"),
-                         (11, "slim"), (12, "slim"), (13, "slim"), (14, "slim"), (15, "slim"), (16, "slim")]:
-        if (tile == 1 and n < 256) or (tile in (9, 10) and n > 16):
+    for tile, kernel in [(1, "walk"), (2, "tile"), (3, "tile"), (4, "tile"), (5, "tile"), (6, "tile"), (7, "tile.once"), (8, "tile.once"), (9, "slim"), (10, "slim"), (11, "slim"), (12, "slim"),
+                         (13, "slim"), (14, "slim"), (15, "staged"), (16, "staged"), (17, "slim.any"), (18, "slim.any"), (19, "slim.any")]:
+        if tile == 1 and n < 256:
             continue
         with G.env(CAMELID_HIP_I8_TILE=tile), G.engaged(f"^i8.matmul.{kernel}$"):
             assert np.array_equal(product(t, q, w, s, ws, bias, q_pad=pad, w_pad=pad), want), tile
 
 
+@pytest.mark.parametrize("n,rows,cols", [(1, 17, 5001), (33, 100, 128), (70, 33, 2057), (300, 700, 131), (16, 300, 1100), (513, 600, 1025)])
+def test_product_of_rows_that_start_anywhere_by_every_kernel(n, rows, cols):
+    q, w, s, ws, bias = operands(n * rows, n, rows, cols)
+    want = want_product("f32", q, w, s, ws, bias)
+    for tile, kernel in [(15, "staged"), (16, "staged"), (17, "slim.any"), (18, "slim.any"), (19, "slim.any")]:
+        for pad, offset in ((0, 0), (3, 1), (-cols % 16, 5)):
+            with G.env(CAMELID_HIP_I8_TILE=tile), G.engaged(f"^i8.matmul.{kernel}$"):
+                assert np.array_equal(product("f32", q, w, s, ws, bias, q_pad=pad, w_pad=pad, offset=offset), want), (tile, pad, offset)
+
+
+@pytest.mark.parametrize("stride", [(1 << 27) + 5, 1 << 27, (1 << 24) + 16, (1 << 24) + 1])
+def test_rows_far_apart(stride):
+    """Offsets past 32 bits."""
+    n, rows, cols = 3, 40, 200
+    q, w, s, ws, _ = operands(5, n, rows, cols)
+    B.init(0)
+    W = B.DeviceBuffer(stride * (rows - 1) + cols)
+    for r in range(rows):
+        check(lib().cml_memcpy_h2d(W.ptr + r * stride, np.ascontiguousarray(w[r]).ctypes.data, cols, None))
+    Q, O, S, WS = Rows(q), Rows.empty(n, rows, BITS["f32"]), f32(s), f32(ws)
+    G.say(f"matmul_i8 rows {stride} bytes apart")
+    check(lib().cml_matmul_i8(Q.ptr, cols, S.ptr, n, W.ptr, stride, WS.ptr, rows, cols, None, TYPES["f32"], O.ptr, rows, None))
+    check(lib().cml_stream_sync(None))
+    assert np.array_equal(O.get(), want_product("f32", q, w, s, ws, None))
+
+
 def test_kernels_by_size():
-    for n, rows, cols, pad, kernel in [(1, 512, 1024, 0, "slim"), (1, 512, 1024, 1, "few"), (40, 512, 1024, 0, "slim"), (400, 4096, 512, 0, "tile"), (40, 512, 1024, 1, "staged"), (40, 98304, 1024, 0, "tile.once"), (2048, 8192, 512, 0, "walk")]:
+    for n, rows, cols, pad, kernel in [(1, 512, 1024, 0, "slim"), (1, 512, 1024, 1, "slim.any"), (40, 512, 1024, 0, "slim"), (400, 4096, 512, 0, "tile"), (40, 512, 1024, 1, "slim.any"), (2000, 2000, 1024, 1, "staged"), (40, 98304, 1024, 0, "tile.once"), (2048, 8192, 512, 0, "walk")]:
         q, w, s, ws, _ = operands(n, n, rows, cols)
         with G.engaged(f"^i8.matmul.{kernel}$"):
             assert np.array_equal(product("f32", q, w, s, ws, None, q_pad=pad, w_pad=pad), want_product("f32", q, w, s, ws, None))
@@ -229,7 +255,7 @@ def test_scales_that_are_not_finite_reach_their_cells_alone():
     assert np.all(np.isfinite(rest))
 
 
-@pytest.mark.parametrize("tile,n,rows,cols", [(0, 5, 300, 512), (0, 300, 700, 512), (1, 600, 1000, 272), (-1, 70, 90, 272)])
+@pytest.mark.parametrize("tile,n,rows,cols", [(0, 5, 300, 512), (0, 300, 700, 512), (1, 600, 1000, 272), (16, 70, 90, 272), (17, 7, 90, 272)])
 def test_the_lane_on_a_stream_and_replayed_from_a_graph(tile, n, rows, cols):
     """Norm and product captured together; every replay on other inputs against the eager calls."""
     import ctypes as C
