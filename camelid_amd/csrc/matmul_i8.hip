@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) 
 //
 // The instruction's 32 rows are the tile's in another order: a lane ends up with 16 neighbouring weight rows of its token and stores them whole.
 //
-// 37 tokens on 128256 x 2048: 50 us, the weight and the logits at 5.6 TB/s.  4096 x 14336 x 4096 (the walk): 222 us, 2.2 POPS; the matrix cores execute 54 % of the busy
+// 37 tokens on 128256 x 2048: 50 us, the weight and the logits at 5.6 TB/s.  4096 x 14336 x 4096 (the walk): 222 us, 2.2 POPS; the matrix cores execute 56 % of the busy
 // cycles, LDS conflicts are gone, and the clock is the limit: under this load it falls from 2.4 to 1.8 GHz (8192 x 8192 x 8192: 451 us, of zeros 335).
 typedef int v16i_i8 __attribute__((ext_vector_type(16)));
 
