@@ -761,10 +761,11 @@ static int cheapest(const MatmulI8 &a, const TileCost (&tiles)[N], float &least)
 static int choose_aligned(const MatmulI8 &a) {
     const int64_t bytes = static_cast<int64_t>(a.rows) * a.cols;
     // A weight of 96 MB and more is used once in a pass over a model: past the caches (128256 x 2048, 1 / 16 / 37 tokens: 52 / 55 / 59 us plain, 45 / 46 / 49 so), in the
-    // tile that has two workgroups for every compute unit (32000 x 4096, 1 / 32 tokens: 128 x 64 31 / 29, 64 x 64 29 / 28; 48 tokens: 30 / 30, plain 24).
+    // tile that has two workgroups for every compute unit (32000 x 4096, 1 / 32 tokens: 128 x 64 31 / 29, 64 x 64 29 / 28; 48 tokens: 30 / 30, plain 24), where that is a tile for every unit
+    // (4096 x 28672, one token: 62, plain and slim 25).
     if (bytes >= 96ll << 20 && a.n_tokens <= 64) {
         if ((a.rows + 127) / 128 >= 512) return 6;
-        if (a.n_tokens <= 32) return 7;
+        if (a.n_tokens <= 32 && (a.rows + 63) / 64 >= 256) return 7;
     }
     float least;
     const int best = cheapest(a, kTiles, least);
