@@ -60,7 +60,7 @@ def compare(t, logits, target, top, **kw):
 # one token; inside, at and past a batch; rows that start off a 16-byte boundary; one row over many parts, many rows of one part
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n,vocab,top,pad,offset", [(1, 1, 1, 0, 0), (3, 2, 5, 0, 0), (2, 63, 64, 1, 0), (5, 1000, 20, 0, 3), (2, 1024, 1, 0, 0), (4, 1025, 20, 0, 0), (1, 2047, 0, 0, 1), (3, 5001, 33, 4, 0),
-                                                    (61, 32003, 5, 1, 0), (1, 128256, 20, 0, 0), (1, 151937, 64, 0, 5), (5000, 300, 3, 1, 0), (4200, 2100, 8, 0, 0)])
+                                                    (61, 32003, 5, 1, 0), (1, 128256, 20, 0, 0), (1, 151937, 64, 0, 5), (5000, 300, 3, 1, 0), (4200, 2100, 8, 0, 0), (1100, 5001, 4, 1, 0), (700, 9001, 6, 0, 0)])
 def test_sizes(t, n, vocab, top, pad, offset):
     rng = np.random.default_rng(vocab + n)
     v = (2 * rng.standard_normal((n, vocab))).astype(np.float32)
