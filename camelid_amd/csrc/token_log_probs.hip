@@ -36,6 +36,7 @@ struct ScoreArgs {
     float *partial;
     int64_t stride, n_rows;
     int vocab, n_top, parts;
+    int depth;             // which of the parts' entries bounds the row's n-th: with twice as many as n of them, half of the parts have n together
     uint32_t top_inverse;  // ceil(2^20 / n_top): i / n_top = i * top_inverse >> 20 for i < 8192
 };
 
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
 }
 
 // The parts of a row, joined: every thread asks for its share of the lists and every wave for the parts' best at once, so that memory is waited for once.  What
-// reaches the n-th largest of the parts' best is gathered in LDS and ranked there (3 instructions for each, an insertion takes 20); the first wave adds the sums up
+// reaches the n-th largest of the parts' best (of their `depth` best, where the parts are few) is gathered in LDS and ranked there (3 instructions for each, an insertion takes 20); the first wave adds the sums up
 // (lane p: parts p and p + 64) and writes.  One row of 126 parts: 5 us with 20 best, 2.6 without a list, most of it the launch and the trip.
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(ScoreArgs a) {
@@ -409,9 +410,10 @@ __global__ __launch_bounds__(kJoinThreads) void token_log_probs_join_kernel(Scor
     const bool here[2] = {lane < a.parts, lane + 64 < a.parts};
     float over = -INFINITY;
     if (a.n_top) {
-        const float best[2] = {here[0] ? p[0][5] : -INFINITY, here[1] ? p[1][5] : -INFINITY};
+        const float bound[2] = {here[0] ? p[0][3 + 2 * a.depth] : -INFINITY, here[1] ? p[1][3 + 2 * a.depth] : -INFINITY};
+        const int enough = (a.n_top + a.depth - 1) / a.depth;
         if (tid == 0) n_found = 0;
-        if (count_above(best, -INFINITY) > a.n_top) over = below_nth(best, a.n_top);
+        if (count_above(bound, -INFINITY) >= enough) over = below_nth(bound, enough);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < kMine; k++)
@@ -488,11 +490,14 @@ size_t token_log_probs_workspace(int64_t n_rows, int64_t vocab, int n_top) {
 
 int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_t n_rows, int64_t vocab, const int32_t *target, int n_top, float *log_prob, int32_t *rank, float *entropy,
                            int32_t *top_ids, float *top_log_probs, void *workspace, hipStream_t st) {
-    int parts = score_parts(n_rows, vocab);
+    const int64_t batch = dtype == CML_F32 ? 1024 : 2048, batches = (vocab + batch - 1) / batch;
+    int parts = static_cast<int>(std::min<int64_t>(score_parts(n_rows, vocab), batches));
     // f32 rows come at memory's rate with fewer waves (20 best of 128256, 1024 rows: two parts 101 us, four 107; 2048: one 186, two 200; 700: two 93, four 77).
     if (dtype == CML_F32 && parts <= 4) parts = static_cast<int>(std::min<int64_t>(parts, std::max<int64_t>(1, 3000 / n_rows)));
     if (parts == 3) parts = 2;
-    const ScoreArgs a{logits, target, log_prob, entropy, top_log_probs, rank, top_ids, static_cast<float *>(workspace), stride, n_rows, static_cast<int>(vocab), n_top, parts,
+    if (parts > 4 && parts <= 8) parts = 4;
+    const int depth = std::max(1, std::min(n_top, (2 * n_top + parts - 1) / parts));
+    const ScoreArgs a{logits, target, log_prob, entropy, top_log_probs, rank, top_ids, static_cast<float *>(workspace), stride, n_rows, static_cast<int>(vocab), n_top, parts, depth,
                       n_top ? ((1u << 20) + n_top - 1) / n_top : 0};
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
