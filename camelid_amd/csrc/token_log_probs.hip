@@ -191,7 +191,15 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
     const int begin = static_cast<int>(static_cast<int64_t>(n_batches) * part / a.parts), end = live ? static_cast<int>(static_cast<int64_t>(n_batches) * (part + 1) / a.parts) : 0;
     Batch<T> ahead;
     const Bits *mine = x + lane * 8;
-    if (begin < end && (begin + 1) * kBatch <= a.vocab) ahead.request(mine + begin * kBatch);
+    // The row's last batch, where it is not whole: of a 16-bit type read from where a whole one ends with the row, what belongs to the batch before masked (one row of 128256 bf16,
+    // 20 best: 13.5 us, logit by logit 15.5); of f32 logit by logit (half as many, and a request behind every batch, whole or not, costs more: 2048 x 128256 186 us and 223).
+    constexpr bool kBack = sizeof(Bits) == 2;
+    const bool fits = kBack && a.vocab >= kBatch;
+    const int last_first = a.vocab - kBatch;
+    if (begin < end) {
+        if (fits) ahead.request(mine + min(begin * kBatch, last_first));
+        else if ((begin + 1) * kBatch <= a.vocab) ahead.request(mine + begin * kBatch);
+    }
     const int target = live ? a.target[row] : -1;
     const bool in_range = target >= 0 && target < a.vocab;
     const float given = in_range ? load_value<T>(x + target) : INFINITY;
@@ -206,10 +214,21 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
         // vmcnt(0): the batch is here.  Said outright, because the compiler, which does not see that no path leaves it in flight, otherwise waits below, at
         // reused registers, for the next batch as well (512 x 128256 bf16 63 us).
         __builtin_amdgcn_s_waitcnt(0x0f70);
-        if (whole) {
+        int first = base;
+        if (fits) {
+            ahead.take(v);
+            if (b + 1 < end) ahead.request(mine + min(base + kBatch, last_first));
+            if (!whole) {
+                first = last_first;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[u][j] = first + (u * 64 + lane) * 8 + j >= base ? v[u][j] : -INFINITY;
+            }
+        } else if (!kBack && whole) {
             ahead.take(v);
             if (b + 1 < end && base + 2 * kBatch <= a.vocab) ahead.request(mine + base + kBatch);
-        } else {  // the row's last batch
+        } else {
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
@@ -226,7 +245,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
         }
         rebase(s, fmaxf(s.most, bm));
         // (instructions bound a row that comes at memory's rate: one less to a logit, and no clamp, is 2048 x 128256 bf16 in 113 us in place of 122)
-        bool plain = !careful && !__builtin_amdgcn_ballot_w64(!(fabsf(s.most) < kOrdinary));
+        bool plain = whole && !careful && !__builtin_amdgcn_ballot_w64(!(fabsf(s.most) < kOrdinary));
         float sum = 0.0f, esum = 0.0f;  // (of this batch: a row's sum is one of few large terms)
         if (plain) {
             const float from = -(s.most * kLog2e);
@@ -273,8 +292,8 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int i = base + (u * 64 + lane) * 8 + j;
-                    s.above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < a.vocab && (v[u][j] > given || (v[u][j] == given && i < target))));
+                    const int i = first + (u * 64 + lane) * 8 + j;
+                    s.above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i >= base && i < a.vocab && (v[u][j] > given || (v[u][j] == given && i < target))));
                 }
         }
         if (a.n_top == 0) continue;
@@ -299,7 +318,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
                     const bool in = v[u][j] > over;
                     const unsigned long long those = __builtin_amdgcn_ballot_w64(in);
                     const int at = count + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(those >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(those), 0));
-                    if (in && at < 64) found[wave][at] = make_uint2(ordered(__float_as_uint(v[u][j])), static_cast<uint32_t>(~(base + (u * 64 + lane) * 8 + j)));
+                    if (in && at < 64) found[wave][at] = make_uint2(ordered(__float_as_uint(v[u][j])), static_cast<uint32_t>(~(first + (u * 64 + lane) * 8 + j)));
                     count += __builtin_popcountll(those);
                 }
             }
@@ -325,7 +344,7 @@ __global__ __launch_bounds__(256) void token_log_probs_kernel(ScoreArgs a) {
                 while (in) {
                     const int from = __builtin_ctzll(in);
                     in &= in - 1;
-                    list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[u][j]), from)), base + (u * 64 + from) * 8 + j);
+                    list_insert(s, ordered(__builtin_amdgcn_readlane(__float_as_uint(v[u][j]), from)), first + (u * 64 + from) * 8 + j);
                 }
             }
         }
