@@ -1,0 +1,36 @@
+"""The int8 lane where f32 ends and where sizes do: squares past the largest f32, an epsilon of 0, rows of no values, very long rows, single rows of any
+stride, more workgroups than one launch may have, and large products cell by cell.
+
+Tolerances are those of the lane's other tests: 4e-6 on scales and normalised values, whatever a row's length; bits elsewhere.
+"""
+import numpy as np
+import pytest
+
+from camelid_amd import binding as B
+from camelid_amd.binding import check, lib
+from tests import gpu_util as G
+from tests.test_gpu_int8_lane import check_norm, f32, norm, operands, product, want_product
+from tests.typed_rows import BITS, TYPES, Rows, from_bits, to_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [4, 600, 5000, 40001])
+def test_squares_past_the_largest_f32_say_so(t, cols):
+    """No quants, a scale and normalised values that are not finite, and nothing of it in the rows beside."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((7, cols)).astype(np.float32)
+    x[1, :4] = [1e20, -5e19, 1e18, 3]  # one square alone
+    x[3] = 0
+    x[3, :4] = 1.2e19                  # each square is finite, their sum is not
+    x[5] = 3e38 * np.sign(x[5])
+    w = (0.5 + rng.random(cols)).astype(np.float32)
+    bits = to_bits(x, t)
+    for residual in (None, np.zeros_like(bits)):
+        s, y, q, d = norm(t, bits, residual, w, 1e-5)
+        bad, good = [1, 3, 5], [0, 2, 4, 6]
+        assert not np.any(np.isfinite(d[bad])) and np.all(q[bad] == 0), (d, q[bad][:, :4])
+        assert np.all(np.isnan(y[bad]))
+        assert np.array_equal(s, bits)
+        check_norm(t, bits[good], None, w, 1e-5, (s[good], y[good], q[good], d[good]))
