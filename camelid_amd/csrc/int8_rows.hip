@@ -38,8 +38,8 @@ template <bool NORM>
 __device__ __forceinline__ RowScale row_scale(const NormRows &a, float sum, uint32_t top) {
     RowScale f;
     const float most = __builtin_bit_cast(float, top);
-    // (squares past the largest f32: 1 / sqrt(inf) is 0, which would make a row of zeros of it)
-    f.inv = !NORM ? 1.0f : sum < INFINITY ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : __builtin_nanf("");
+    // (squares past the largest f32: 1 / sqrt(inf) is 0, which would make a row of zeros of it; a row of zeros is one whatever eps says, and 0 / 0 is none)
+    f.inv = !NORM ? 1.0f : most == 0.0f ? 0.0f : sum < INFINITY ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : __builtin_nanf("");
     f.scale = most * f.inv / 127.0f;
     f.lift = most < 1e-30f ? 18446744073709551616.0f : 1.0f;  // 127 / most of a row of tiny values would be infinite: such a row is lifted by 2^64 first
     f.live = most > 0.0f && fabsf(f.scale) < INFINITY;       // a row of zeros, or one that leaves f32 (its scale is NaN or infinite): no quants

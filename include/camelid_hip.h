@@ -431,8 +431,10 @@ int cml_moe_weighted_sum(const float *y_dev, const int32_t *route_to_assignment_
  *   y = h * weight / sqrt(mean(h^2) + eps) -> normed_dev (f32[n_tokens*cols], nullable)
  *   scale = max|y| / 127 -> scales_dev f32[n_tokens];  round(y / scale), ties to even -> q_dev
  * residual_dev null: h = x.  weight_dev f32[cols].  Sums in f32.  A row of zeros has scale 0 and quants
- * 0; a row whose values or squares, or the sum of those, leave the finite f32 numbers (values from about 1e18 on do) has
- * scale NaN or infinite and quants 0, and where it is the squares, normalised values of NaN.  Rows of up to 2^24 values (beyond 32768 at a lower speed). */
+ * 0, for any eps; a row whose values or squares, or the sum of those, leave the finite f32 numbers (values from about 1e18 on do) has
+ * scale NaN or infinite and quants 0, and where it is the squares, normalised values of NaN.  eps may be 0; then the squares
+ * are what there is: a row that is not zero but whose squares all vanish (values below 1e-23) has an infinite scale and quants 0, and one
+ * whose squares are subnormal (below 1e-19) loses bits.  Rows of up to 2^24 values (beyond 32768 at a lower speed). */
 int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const void *residual_dev,
                         int64_t residual_stride, const float *weight_dev, float eps, int64_t n_tokens,
                         int64_t cols, void *sum_dev, int64_t sum_stride, float *normed_dev,

@@ -34,3 +34,23 @@ def test_squares_past_the_largest_f32_say_so(t, cols):
         assert np.all(np.isnan(y[bad]))
         assert np.array_equal(s, bits)
         check_norm(t, bits[good], None, w, 1e-5, (s[good], y[good], q[good], d[good]))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols", [1, 600, 5000, 40001])
+def test_an_epsilon_of_zero(t, cols):
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((5, cols)).astype(np.float32)
+    x[1] = 0
+    x[3] = -0.0
+    r = np.zeros_like(x)
+    r[4] = -from_bits(to_bits(x[4], t), t)  # the residual takes it all away
+    w = (0.5 + rng.random(cols)).astype(np.float32)
+    s, y, q, d = norm(t, to_bits(x, t), to_bits(r, t), w, 0.0)
+    zero = [1, 3, 4]
+    assert np.all(d[zero] == 0) and np.all(q[zero] == 0) and np.all(y[zero] == 0), d
+    check_norm(t, to_bits(x[[0, 2]], t), None, w, 0.0, (s[[0, 2]], y[[0, 2]], q[[0, 2]], d[[0, 2]]))
+    if t != "f16":  # squares that all vanish: not a row of zeros, and no scale that could be given
+        tiny = np.full((1, cols), 1e-30, np.float32)
+        _, y, q, d = norm(t, to_bits(tiny, t), None, w, 0.0)
+        assert not np.isfinite(d[0]) and np.all(q == 0)
