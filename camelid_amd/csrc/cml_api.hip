@@ -739,7 +739,10 @@ int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const vo
     if (int rc = check_ready()) return rc;
     if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
     if (n_tokens < 0 || cols < 0 || n_tokens > kMostRows) return fail(CML_ERR_SHAPE, "%lld rows of %lld values", (long long)n_tokens, (long long)cols);
-    if (n_tokens == 0 || cols == 0) return CML_OK;
+    if (n_tokens == 0) return CML_OK;
+    if (int rc = bad_f32("scales", scales_dev)) return rc;
+    // (rows of no values: nothing is read, and every scale is 0)
+    if (cols == 0) return launch_add_rms_norm_i8(dtype, nullptr, 0, nullptr, 0, nullptr, eps, n_tokens, 0, nullptr, 0, nullptr, nullptr, 0, scales_dev, as_stream(stream));
     if (cols > kMostI8Row) return fail(CML_ERR_UNSUPPORTED, "a row of %lld values: at most %lld", (long long)cols, (long long)kMostI8Row);
     const int bytes = type_bytes(dtype);
     if (int rc = bad_rows("x", x_dev, x_stride, cols, n_tokens, bytes)) return rc;
@@ -749,7 +752,6 @@ int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const vo
         if (int rc = bad_rows("sum", sum_dev, sum_stride, cols, n_tokens, bytes)) return rc;
     if (int rc = bad_rows("q", q_dev, q_stride, cols, n_tokens, 1)) return rc;
     if (int rc = bad_f32("weight", weight_dev)) return rc;
-    if (int rc = bad_f32("scales", scales_dev)) return rc;
     if (normed_dev)
         if (int rc = bad_f32("normed", normed_dev)) return rc;
     return launch_add_rms_norm_i8(dtype, x_dev, x_stride, residual_dev, residual_stride, weight_dev, eps, n_tokens, cols, sum_dev, sum_stride, normed_dev, q_dev, q_stride, scales_dev,
@@ -760,11 +762,12 @@ int cml_quantize_i8(int dtype, const void *x_dev, int64_t x_stride, int64_t n_ro
     if (int rc = check_ready()) return rc;
     if (!known_type(dtype)) return fail(CML_ERR_INVALID, "unknown value type %d", dtype);
     if (n_rows < 0 || cols < 0 || n_rows > kMostRows) return fail(CML_ERR_SHAPE, "%lld rows of %lld values", (long long)n_rows, (long long)cols);
-    if (n_rows == 0 || cols == 0) return CML_OK;
+    if (n_rows == 0) return CML_OK;
+    if (int rc = bad_f32("scales", scales_dev)) return rc;
+    if (cols == 0) return launch_quantize_i8(dtype, nullptr, 0, n_rows, 0, nullptr, 0, scales_dev, as_stream(stream));  // (every scale is 0)
     if (cols > kMostI8Row) return fail(CML_ERR_UNSUPPORTED, "a row of %lld values: at most %lld", (long long)cols, (long long)kMostI8Row);
     if (int rc = bad_rows("x", x_dev, x_stride, cols, n_rows, type_bytes(dtype))) return rc;
     if (int rc = bad_rows("q", q_dev, q_stride, cols, n_rows, 1)) return rc;
-    if (int rc = bad_f32("scales", scales_dev)) return rc;
     return launch_quantize_i8(dtype, x_dev, x_stride, n_rows, cols, q_dev, q_stride, scales_dev, as_stream(stream));
 }
 

@@ -434,12 +434,14 @@ int cml_moe_weighted_sum(const float *y_dev, const int32_t *route_to_assignment_
  * 0, for any eps; a row whose values or squares, or the sum of those, leave the finite f32 numbers (values from about 1e18 on do) has
  * scale NaN or infinite and quants 0, and where it is the squares, normalised values of NaN.  eps may be 0; then the squares
  * are what there is: a row that is not zero but whose squares all vanish (values below 1e-23) has an infinite scale and quants 0, and one
- * whose squares are subnormal (below 1e-19) loses bits.  Rows of up to 2^24 values (beyond 32768 at a lower speed). */
+ * whose squares are subnormal (below 1e-19) loses bits.  Rows of up to 2^24 values (beyond 32768 at a lower speed); rows of no values have
+ * scale 0, and only scales_dev is looked at. */
 int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const void *residual_dev,
                         int64_t residual_stride, const float *weight_dev, float eps, int64_t n_tokens,
                         int64_t cols, void *sum_dev, int64_t sum_stride, float *normed_dev,
                         int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream);
-/* The quantizer alone, y = x: activations that no norm precedes, and weights (one scale per weight row). */
+/* The quantizer alone, y = x: activations that no norm precedes, and weights (one scale per weight row).  Zeros, infinities, NaN and rows
+ * of no values as above. */
 int cml_quantize_i8(int dtype, const void *x_dev, int64_t x_stride, int64_t n_rows, int64_t cols,
                     int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream);
 /* q * scale, rounded to dtype. */
@@ -447,7 +449,7 @@ int cml_dequantize_i8(const int8_t *q_dev, int64_t q_stride, const float *scales
                       int64_t cols, int dtype, void *out_dev, int64_t out_stride, cml_stream_t stream);
 /* out[t][r] = (sum over c of q[t][c] * w[r][c]) * scales[t] * w_scales[r] + bias[r], the sum an exact
  * 32-bit integer, the rest in f32, rounded once to dtype.  q int8[n_tokens][cols], w int8[rows][cols]
- * (any of the 256 values), bias_dev f32[rows] or null.  cols up to 131071.  The bits depend neither on the
+ * (any of the 256 values), bias_dev f32[rows] or null.  cols from 1 to 131071 (rows of no values are refused).  The bits depend neither on the
  * number of tokens nor on the kernel that serves the call.  Rows that start on 16-byte boundaries (base and stride, of q and
  * w both) run on the faster kernels. */
 int cml_matmul_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev, int64_t n_tokens,

@@ -54,3 +54,22 @@ def test_an_epsilon_of_zero(t, cols):
         tiny = np.full((1, cols), 1e-30, np.float32)
         _, y, q, d = norm(t, to_bits(tiny, t), None, w, 0.0)
         assert not np.isfinite(d[0]) and np.all(q == 0)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_rows_of_no_values_have_scale_zero(t):
+    B.init(0)
+    n = 700
+    x, q, w, D = Rows.empty(1, 8, BITS[t]), Rows.empty(1, 8, np.int8), f32(np.ones(1)), Rows.empty(1, n, np.float32)
+    G.say(f"quantize_i8 / add_rms_norm_i8 {t} {n}x0")
+    check(lib().cml_quantize_i8(TYPES[t], x.ptr, 0, n, 0, q.ptr, 0, D.ptr, None))
+    check(lib().cml_stream_sync(None))
+    assert np.all(D.get() == 0)
+    D = Rows.empty(1, n, np.float32)
+    check(lib().cml_add_rms_norm_i8(TYPES[t], x.ptr, 0, x.ptr, 0, w.ptr, 0.0, n, 0, x.ptr, 0, None, q.ptr, 0, D.ptr, None))
+    check(lib().cml_stream_sync(None))
+    assert np.all(D.get() == 0)
+    assert np.all(x.get().view(np.uint8) == 0xA5) and np.all(q.get().view(np.uint8) == 0xA5)  # (nothing else was written)
+    assert lib().cml_quantize_i8(TYPES[t], x.ptr, 0, n, 0, q.ptr, 0, None, None) == 2
+    assert lib().cml_quantize_i8(TYPES[t], None, 0, n, 0, None, 0, D.ptr, None) == 0  # (nothing to read, nothing else to write)
+    check(lib().cml_stream_sync(None))
