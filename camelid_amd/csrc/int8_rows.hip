@@ -5,7 +5,7 @@
 //   scale = max|y| / 127, q = round(y / scale), ties to even
 //
 // A row stays in registers between its one read and its writes.  The quotient y / scale is h * weight * (127 / max|h * weight|): inv cancels, so
-// the sum of squares and the maximum are reduced together, behind one barrier.  Sums and products are f32; the only roundings to
+// the sum of squares and the maximum are reduced together, behind one barrier.  Sums (of up to 32 squares a thread; longer rows in 64 bits) and products are f32; the only roundings to
 // fewer bits are the stream's type and the 8 bits themselves.
 //
 // Memory's rate bounds long prompts: 8192 x 4096 bf16 in 45 us (5.2 TB/s; a large copy 5.2), read back in 18 (5.5).  One token: 2.7 us, a launch.
@@ -168,7 +168,8 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rows_to_i8_kern
     }
 }
 
-// Rows that the registers do not hold: read twice, the second time from `sum` where it is written (which may be x or residual).
+// Rows that the registers do not hold: read twice, the second time from `sum` where it is written (which may be x or residual).  A thread adds up to 16384 squares, one
+// after the other: in 64 bits, because in 32 their roundings, which all go one way where values are alike, come to 1e-4 of the inverse root.
 template <class T, bool NORM>
 __global__ __launch_bounds__(1024) void long_rows_to_i8_kernel(NormRows a) {
     typedef typename T::Bits Bits;
@@ -183,15 +184,15 @@ __global__ __launch_bounds__(1024) void long_rows_to_i8_kernel(NormRows a) {
         const float v = load_value<T>(x + i);
         return r ? rounded<T>(v + load_value<T>(r + i)) : v;
     };
-    float sum = 0.0f;
+    double squares = 0.0;
     uint32_t top = 0;
     for (int i = tid; i < a.cols; i += 1024) {
         const float h = value(i);
         if (out) store_value<T>(out + i, h);
-        if (NORM) sum = fmaf(h, h, sum);
+        if (NORM) squares = fma(static_cast<double>(h), static_cast<double>(h), squares);
         top = max(top, __builtin_bit_cast(uint32_t, NORM ? h * a.weight[i] : h) & 0x7fffffffu);
     }
-    sum = wave_allsum(sum);
+    float sum = wave_allsum(static_cast<float>(squares));
     top = static_cast<uint32_t>(wave_allmax_i32(static_cast<int>(top)));
     if ((tid & 63) == 0) {
         s_sum[tid >> 6] = sum;

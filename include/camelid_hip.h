@@ -430,7 +430,7 @@ int cml_moe_weighted_sum(const float *y_dev, const int32_t *route_to_assignment_
  *   h = x + residual, rounded to dtype     -> sum_dev (nullable; may be x or residual itself)
  *   y = h * weight / sqrt(mean(h^2) + eps) -> normed_dev (f32[n_tokens*cols], nullable)
  *   scale = max|y| / 127 -> scales_dev f32[n_tokens];  round(y / scale), ties to even -> q_dev
- * residual_dev null: h = x.  weight_dev f32[cols].  Sums in f32.  A row of zeros has scale 0 and quants
+ * residual_dev null: h = x.  weight_dev f32[cols].  Sums in f32 (a thread's part of a row over 32768 values in f64).  A row of zeros has scale 0 and quants
  * 0, for any eps; a row whose values or squares, or the sum of those, leave the finite f32 numbers (values from about 1e18 on do) has
  * scale NaN or infinite and quants 0, and where it is the squares, normalised values of NaN.  eps may be 0; then the squares
  * are what there is: a row that is not zero but whose squares all vanish (values below 1e-23) has an infinite scale and quants 0, and one

@@ -73,3 +73,14 @@ def test_rows_of_no_values_have_scale_zero(t):
     assert lib().cml_quantize_i8(TYPES[t], x.ptr, 0, n, 0, q.ptr, 0, None, None) == 2
     assert lib().cml_quantize_i8(TYPES[t], None, 0, n, 0, None, 0, D.ptr, None) == 0  # (nothing to read, nothing else to write)
     check(lib().cml_stream_sync(None))
+
+
+@pytest.mark.parametrize("t,cols", [("f32", 1 << 22), ("bf16", (1 << 22) + 3), ("f32", 1 << 24)])
+@pytest.mark.parametrize("value", [0.7, 1.1, 2.7])
+def test_very_long_rows_of_values_alike(t, cols, value):
+    """Roundings of a running sum all go one way here."""
+    rng = np.random.default_rng(1)
+    x = (value * (1 + 1e-6 * rng.standard_normal((1, cols)))).astype(np.float32)
+    w = np.ones(cols, np.float32)
+    bits = to_bits(x, t)
+    check_norm(t, bits, None, w, 1e-5, norm(t, bits, None, w, 1e-5))
