@@ -732,7 +732,7 @@ static int bad_f32(const char *what, const void *p) {
 }
 constexpr int64_t kMostI8Row = 1 << 24;    // values of a row that one workgroup quantizes
 constexpr int64_t kMostI8Cols = 131071;    // |sum| <= 2^14 * cols stays below 2^31
-constexpr int64_t kMostRows = 1 << 30;     // rows or tokens of one call: a grid's workgroups are counted in 31 bits
+constexpr int64_t kMostRows = 1 << 30;     // rows or tokens of one call (in as many launches as their workgroups take)
 
 int cml_add_rms_norm_i8(int dtype, const void *x_dev, int64_t x_stride, const void *residual_dev, int64_t residual_stride, const float *weight_dev, float eps, int64_t n_tokens,
                         int64_t cols, void *sum_dev, int64_t sum_stride, float *normed_dev, int8_t *q_dev, int64_t q_stride, float *scales_dev, cml_stream_t stream) {

@@ -6,6 +6,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <atomic>
 #include <string>
 
@@ -220,5 +221,11 @@ int launch_token_log_probs(int dtype, const void *logits, int64_t stride, int64_
 
 // Integer tuning knob read once from the environment (0 when unset).
 int env_int(const char *name, int dflt);
+
+// Workgroups of `threads` that one launch may have: it counts its work items in 32 bits.  More rows than that go in several launches.
+inline int64_t most_workgroups(int threads) {
+    const int items = env_int("CAMELID_HIP_LAUNCH_ITEMS", 0);
+    return std::max<int64_t>(1, (items > 0 ? items : (1ll << 32) - 1) / threads);
+}
 
 }  // namespace cml

@@ -11,6 +11,8 @@
 // Memory's rate bounds long prompts: 8192 x 4096 bf16 in 45 us (5.2 TB/s; a large copy 5.2), read back in 18 (5.5).  One token: 2.7 us, a launch.
 #include "typed_rows.hpp"
 
+#include <algorithm>
+
 #pragma clang fp contract(off)
 
 namespace cml {
@@ -241,17 +243,39 @@ static int launch_rows_typed(const NormRows &a, hipStream_t st) {
     return CML_OK;
 }
 
+// Rows in as many launches as workgroups of 1024, the largest, allow.
+template <bool NORM>
+static int launch_all_rows(int dtype, const NormRows &a, hipStream_t st) {
+    const int64_t most = most_workgroups(1024);
+    return with_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        typedef typename T::Bits Bits;
+        for (int64_t first = 0; first < a.n_rows; first += most) {
+            NormRows part = a;
+            part.x = static_cast<const Bits *>(a.x) + first * a.x_stride;
+            if (a.residual) part.residual = static_cast<const Bits *>(a.residual) + first * a.residual_stride;
+            if (a.sum) part.sum = static_cast<Bits *>(a.sum) + first * a.sum_stride;
+            if (a.normed) part.normed = a.normed + first * a.cols;
+            part.q = a.q + first * a.q_stride;
+            part.scales = a.scales + first;
+            part.n_rows = std::min(most, a.n_rows - first);
+            if (NORM) CML_COUNT_LAUNCH("i8.add_rms_norm");
+            else CML_COUNT_LAUNCH("i8.quantize");
+            if (int rc = launch_rows_typed<T, NORM>(part, st)) return rc;
+        }
+        return CML_OK;
+    });
+}
+
 int launch_add_rms_norm_i8(int dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const float *weight, float eps, int64_t n_tokens, int64_t cols,
                            void *sum, int64_t sum_stride, float *normed, int8_t *q, int64_t q_stride, float *scales, hipStream_t st) {
     const NormRows a{x, residual, weight, sum, normed, q, scales, x_stride, residual_stride, sum_stride, q_stride, n_tokens, static_cast<int>(cols), eps};
-    CML_COUNT_LAUNCH("i8.add_rms_norm");
-    return with_type(dtype, [&](auto t) { return launch_rows_typed<decltype(t), true>(a, st); });
+    return launch_all_rows<true>(dtype, a, st);
 }
 
 int launch_quantize_i8(int dtype, const void *x, int64_t x_stride, int64_t n_rows, int64_t cols, int8_t *q, int64_t q_stride, float *scales, hipStream_t st) {
     const NormRows a{x, nullptr, nullptr, nullptr, nullptr, q, scales, x_stride, 0, 0, q_stride, n_rows, static_cast<int>(cols), 0.0f};
-    CML_COUNT_LAUNCH("i8.quantize");
-    return with_type(dtype, [&](auto t) { return launch_rows_typed<decltype(t), false>(a, st); });
+    return launch_all_rows<false>(dtype, a, st);
 }
 
 // out = q * scale, sixteen values a thread.
@@ -281,12 +305,15 @@ __global__ __launch_bounds__(256) void dequantize_i8_kernel(const int8_t *__rest
 
 int launch_dequantize_i8(const int8_t *q, int64_t q_stride, const float *scales, int64_t n_rows, int64_t cols, int dtype, void *out, int64_t out_stride, hipStream_t st) {
     const int chunks = static_cast<int>((cols + 4095) / 4096);
-    CML_COUNT_LAUNCH("i8.dequantize");
+    const int64_t most = std::max<int64_t>(1, most_workgroups(256) / chunks);
     return with_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL(dequantize_i8_kernel<T>, dim3(static_cast<unsigned>(n_rows * chunks)), dim3(256), 0, st, q, q_stride, scales, static_cast<int>(cols), chunks,
-                           static_cast<typename T::Bits *>(out), out_stride);
-        CML_HIP_TRY(hipGetLastError());
+        for (int64_t first = 0; first < n_rows; first += most) {
+            CML_COUNT_LAUNCH("i8.dequantize");
+            hipLaunchKernelGGL(dequantize_i8_kernel<T>, dim3(static_cast<unsigned>(std::min(most, n_rows - first) * chunks)), dim3(256), 0, st, q + first * q_stride, q_stride, scales + first,
+                               static_cast<int>(cols), chunks, static_cast<typename T::Bits *>(out) + first * out_stride, out_stride);
+            CML_HIP_TRY(hipGetLastError());
+        }
         return CML_OK;
     });
 }

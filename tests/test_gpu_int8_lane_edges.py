@@ -84,3 +84,45 @@ def test_very_long_rows_of_values_alike(t, cols, value):
     w = np.ones(cols, np.float32)
     bits = to_bits(x, t)
     check_norm(t, bits, None, w, 1e-5, norm(t, bits, None, w, 1e-5))
+
+
+def launched(call, name):
+    before = G.launch_counts().get(name, 0)
+    out = call()
+    return out, G.launch_counts().get(name, 0) - before
+
+
+def test_more_rows_than_one_launch_has_workgroups():
+    """A launch has fewer than 2^32 work items: 2^24 workgroups of 256 are one too many."""
+    B.init(0)
+    n, cols = (1 << 24) + 5, 3
+    rng = np.random.default_rng(0)
+    q, d = rng.integers(-127, 128, (n, cols)).astype(np.int8), rng.random(n).astype(np.float32)
+    Q, D, O = Rows(q), Rows(d.reshape(1, -1)), Rows.empty(n, cols, np.uint32)
+    G.say(f"dequantize_i8 {n}x{cols}")
+    check(lib().cml_dequantize_i8(Q.ptr, cols, D.ptr, n, cols, 0, O.ptr, cols, None))
+    check(lib().cml_stream_sync(None))
+    assert np.array_equal(O.get(), to_bits(q.astype(np.float32) * d[:, None], "f32"))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n,cols", [(300, 40), (37, 700), (29, 3000), (21, 6000), (11, 17000), (9, 20001), (7, 33000)])
+def test_rows_in_several_launches(t, n, cols):
+    """With a limit of four workgroups of 1024: the same bits, in as many launches as that makes."""
+    rng = np.random.default_rng(n)
+    x, r = to_bits(rng.standard_normal((n, cols)), t), to_bits(rng.standard_normal((n, cols)), t)
+    w = (0.5 + rng.random(cols)).astype(np.float32)
+    want = norm(t, x, r, w, 1e-5, pad=1)
+    with G.env(CAMELID_HIP_LAUNCH_ITEMS=4096):
+        got, launches = launched(lambda: norm(t, x, r, w, 1e-5, pad=1), "i8.add_rms_norm")
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
+    assert launches > 1
+    q, d = want[2], want[3]
+    Q, D, O, P = Rows(q, cols + 1), Rows(d.reshape(1, -1)), Rows.empty(n, cols, BITS[t], cols + 2), Rows.empty(n, cols, np.int8)
+    with G.env(CAMELID_HIP_LAUNCH_ITEMS=4096):
+        _, launches = launched(lambda: check(lib().cml_dequantize_i8(Q.ptr, cols + 1, D.ptr, n, cols, TYPES[t], O.ptr, cols + 2, None)), "i8.dequantize")
+        check(lib().cml_quantize_i8(TYPES[t], O.ptr, cols + 2, n, cols, P.ptr, cols, D.ptr, None))
+    check(lib().cml_stream_sync(None))
+    assert np.array_equal(O.get(), to_bits(q.astype(np.float32) * d[:, None], t)) and launches > 1
+    assert np.all(np.abs(P.get().astype(int)).max(axis=1) == 127)
