@@ -13,6 +13,7 @@
 // A token has a whole wave, or 16 lanes of one.  A group has 1, 2, 4, 8 or 16 lanes and each of them NE neighbouring experts (the group's last ones fewer or none):
 // what is ahead in lane and place has the lower index.  With 16 lanes for a token each has the experts of four, and adds them up as four, so that both forms give the
 // same bits.
+#include <algorithm>
 #include <type_traits>
 
 #include "typed_rows.hpp"
@@ -372,8 +373,16 @@ static int launch_route(RouteArgs a, hipStream_t st) {
 int launch_moe_route_scored(int score, int dtype, const void *logits, int64_t stride, const float *bias, int64_t n_tokens, int n_experts, int n_groups, int groups_kept, int group_top, int k,
                             int renormalise, float weight_scale, int32_t *idx, float *weight, hipStream_t st) {
     const int size = n_experts / n_groups;
-    const RouteArgs a{logits, bias, idx, weight, stride, n_tokens, n_experts, n_groups, groups_kept, group_top, k, size, 0, renormalise, weight_scale};
-    return with_type(dtype, [&](auto t) { return score == CML_ROUTE_SIGMOID ? launch_route<decltype(t), true>(a, st) : launch_route<decltype(t), false>(a, st); });
+    const int64_t most = 4 * most_workgroups(256);  // tokens of a launch, a wave each
+    return with_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        for (int64_t first = 0; first < n_tokens; first += most) {
+            const RouteArgs a{static_cast<const typename T::Bits *>(logits) + first * stride, bias, idx + first * k, weight + first * k, stride, std::min(most, n_tokens - first), n_experts, n_groups,
+                              groups_kept, group_top, k, size, 0, renormalise, weight_scale};
+            if (int rc = score == CML_ROUTE_SIGMOID ? launch_route<T, true>(a, st) : launch_route<T, false>(a, st)) return rc;
+        }
+        return CML_OK;
+    });
 }
 
 }  // namespace cml
