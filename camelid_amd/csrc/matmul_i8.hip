@@ -663,6 +663,23 @@ inline TileGrid tile_grid(const MatmulI8 &a, int rows, int tokens) {
     return TileGrid{(a.rows + rows - 1) / rows, n, std::min(4, n)};
 }
 
+// Calls launch(part) for as many of the tokens at a time, in whole tiles of `tokens`, as a launch has workgroups of `threads` for; row_blocks of them take a token block
+// (and seven blocks more, where a grid has them in eights).
+template <class T, class F>
+static int over_tokens(const MatmulI8 &a, int64_t row_blocks, int tokens, int threads, F launch) {
+    const int64_t most = std::max<int64_t>(1, most_workgroups(threads) / row_blocks - 7) * tokens;
+    for (int64_t first = 0; first < a.n_tokens; first += most) {
+        MatmulI8 part = a;
+        part.q = a.q + first * a.q_stride;
+        part.scales = a.scales + first;
+        part.out = static_cast<typename T::Bits *>(a.out) + first * a.out_stride;
+        part.n_tokens = static_cast<int>(std::min<int64_t>(most, a.n_tokens - first));
+        launch(part);
+        CML_HIP_TRY(hipGetLastError());
+    }
+    return CML_OK;
+}
+
 template <class T, int WR, int WT, int MT, int NT, int STAGES, int PER_CU, bool ONCE = false>
 static int launch_tile(const MatmulI8 &a, hipStream_t st) {
     typedef TileWork<T, WR, WT, MT, NT, STAGES, ONCE, false> Work;
@@ -670,23 +687,26 @@ static int launch_tile(const MatmulI8 &a, hipStream_t st) {
     const auto kernel = matmul_i8_tile_kernel<T, WR, WT, MT, NT, STAGES, PER_CU, ONCE>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
-    const TileGrid grid = tile_grid(a, Work::kRows, Work::kTokens);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid.n_row_blocks * grid.n_token_blocks)), dim3(Work::kThreads), Work::kLds, st, a, grid);
-    CML_HIP_TRY(hipGetLastError());
-    return CML_OK;
+    return over_tokens<T>(a, (a.rows + Work::kRows - 1) / Work::kRows, Work::kTokens, Work::kThreads, [&](const MatmulI8 &part) {
+        const TileGrid grid = tile_grid(part, Work::kRows, Work::kTokens);
+        CML_COUNT_LAUNCH(ONCE ? "i8.matmul.tile.once" : "i8.matmul.tile");
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid.n_row_blocks * grid.n_token_blocks)), dim3(Work::kThreads), Work::kLds, st, part, grid);
+    });
 }
 
 template <class T, int RT, int TT, int WAVES, int STAGES, bool ANY>
 static int launch_slim(const MatmulI8 &a, hipStream_t st) {
     constexpr int kLds = WAVES * STAGES * 16 * (RT + TT) * 128;
     static_assert(kLds <= 160 * 1024 && kLds >= RT * TT * WAVES * 1024, "LDS");
-    const int n_row_blocks = (a.rows + 16 * RT - 1) / (16 * RT), n_columns = (a.n_tokens + 16 * TT - 1) / (16 * TT);
+    const int n_row_blocks = (a.rows + 16 * RT - 1) / (16 * RT);
     const auto kernel = matmul_i8_slim_kernel<T, RT, TT, WAVES, STAGES, ANY>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, kLds, raised)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(a.rows >= a.n_tokens ? wide_grid(n_row_blocks, n_columns) : wide_grid(n_columns, n_row_blocks)), dim3(64 * WAVES), kLds, st, a);
-    CML_HIP_TRY(hipGetLastError());
-    return CML_OK;
+    return over_tokens<T>(a, n_row_blocks + 7, 16 * TT, 64 * WAVES, [&](const MatmulI8 &part) {
+        const int n_columns = (part.n_tokens + 16 * TT - 1) / (16 * TT);
+        CML_COUNT_LAUNCH(ANY ? "i8.matmul.slim.any" : "i8.matmul.slim");
+        hipLaunchKernelGGL(kernel, dim3(part.rows >= part.n_tokens ? wide_grid(n_row_blocks, n_columns) : wide_grid(n_columns, n_row_blocks)), dim3(64 * WAVES), kLds, st, part);
+    });
 }
 
 template <class T, int MT>
@@ -695,10 +715,11 @@ static int launch_staged(const MatmulI8 &a, hipStream_t st) {
     const auto kernel = matmul_i8_staged_kernel<T, MT>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
-    const TileGrid grid = tile_grid(a, Work::kRows, Work::kTokens);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid.n_row_blocks * grid.n_token_blocks)), dim3(Work::kThreads), Work::kLds, st, a, grid);
-    CML_HIP_TRY(hipGetLastError());
-    return CML_OK;
+    return over_tokens<T>(a, (a.rows + Work::kRows - 1) / Work::kRows, Work::kTokens, Work::kThreads, [&](const MatmulI8 &part) {
+        const TileGrid grid = tile_grid(part, Work::kRows, Work::kTokens);
+        CML_COUNT_LAUNCH("i8.matmul.staged");
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid.n_row_blocks * grid.n_token_blocks)), dim3(Work::kThreads), Work::kLds, st, part, grid);
+    });
 }
 
 template <class T, bool STREAM>
@@ -707,6 +728,7 @@ static int launch_walk_stores(const MatmulI8 &a, hipStream_t st) {
     const auto kernel = matmul_i8_walk_kernel<T, 2, 4, 4, 2, STREAM>;
     static std::atomic<bool> raised{false};
     if (int rc = allow_lds(kernel, Work::kLds, raised)) return rc;
+    CML_COUNT_LAUNCH("i8.matmul.walk");
     hipLaunchKernelGGL(kernel, dim3(256), dim3(Work::kThreads), Work::kLds, st, a, tile_grid(a, Work::kRows, Work::kTokens));
     CML_HIP_TRY(hipGetLastError());
     return CML_OK;
@@ -812,12 +834,6 @@ int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int
     const bool near = q_stride < (1 << 26) && w_stride < (1 << 26);  // (64 rows within 32 bits)
     int v = aligned ? choose_aligned(a) : near ? choose_any(a) : 15;
     if (near && forced >= (aligned ? 0 : 14) && forced <= 18 && !(forced == 0 && (rows < 256 || n_tokens < 256))) v = forced;
-    if (v == 0) CML_COUNT_LAUNCH("i8.matmul.walk");
-    else if (v < 6) CML_COUNT_LAUNCH("i8.matmul.tile");
-    else if (v < 8) CML_COUNT_LAUNCH("i8.matmul.tile.once");
-    else if (v < 14) CML_COUNT_LAUNCH("i8.matmul.slim");
-    else if (v < 16) CML_COUNT_LAUNCH("i8.matmul.staged");
-    else CML_COUNT_LAUNCH("i8.matmul.slim.any");
     return with_type(dtype, [&](auto t) { return launch_variant<decltype(t)>(v, a, st); });
 }
 

@@ -420,7 +420,8 @@ int cml_moe_weighted_sum(const float *y_dev, const int32_t *route_to_assignment_
 
 /* ==== the int8 lane and scoring ================================================================
  * Rows of f32, f16 or bf16 values (`dtype`: the GGUF type ids below), strides in elements between the
- * starts of rows (at least the row's length), any element-aligned address.  None of these has a
+ * starts of rows (at least the row's length), any element-aligned address.  Up to 2^30 rows or tokens a call; the product takes up to
+ * 2^20 tokens, 2^27 rows and 2^37 outputs, scoring up to 2^24 rows.  None of these has a
  * counterpart in the reference, whose activations are f32 and whose 8-bit forms scale blocks. */
 #define CML_F32 0
 #define CML_F16 1

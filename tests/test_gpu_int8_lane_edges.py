@@ -126,3 +126,15 @@ def test_rows_in_several_launches(t, n, cols):
     check(lib().cml_stream_sync(None))
     assert np.array_equal(O.get(), to_bits(q.astype(np.float32) * d[:, None], t)) and launches > 1
     assert np.all(np.abs(P.get().astype(int)).max(axis=1) == 127)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n,rows,cols,pad", [(1100, 200, 256, 0), (1100, 200, 256, 1), (300, 3000, 130, 0), (300, 3000, 130, 14), (2100, 33, 1040, 0)])
+def test_tokens_in_several_launches(t, n, rows, cols, pad):
+    q, w, s, ws, bias = operands(n, n, rows, cols)
+    for tile in (0, 2, 4, 6, 11, 15, 16, 19):  # (a variant that does not serve the call is not taken)
+        with G.env(CAMELID_HIP_I8_TILE=tile, CAMELID_HIP_LAUNCH_ITEMS=1 << 13):
+            got, launches = launched(lambda: product(t, q, w, s, ws, bias, q_pad=pad, w_pad=pad, out_pad=3), "i8.matmul.staged")
+        assert np.array_equal(got, want_product(t, q, w, s, ws, bias)), tile
+        if tile == 16:
+            assert launches > 1
