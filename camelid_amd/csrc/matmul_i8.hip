@@ -827,6 +827,9 @@ static int launch_variant(int v, const MatmulI8 &a, hipStream_t st) {
 
 int launch_matmul_i8(const int8_t *q, int64_t q_stride, const float *scales, int64_t n_tokens, const int8_t *w, int64_t w_stride, const float *w_scales, int64_t rows, int64_t cols,
                      const float *bias, int dtype, void *out, int64_t out_stride, hipStream_t st) {
+    // (the stride of a single row says nothing: whatever a caller has there, the row's address decides)
+    if (n_tokens == 1) q_stride = 0;
+    if (rows == 1) w_stride = 0;
     const MatmulI8 a{q, w, scales, w_scales, bias, out, q_stride, w_stride, out_stride, static_cast<int>(n_tokens), static_cast<int>(rows), static_cast<int>(cols)};
     const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(w) | static_cast<uintptr_t>(q_stride | w_stride)) & 15u) == 0 &&
                          q_stride < (1 << 23) && w_stride < (1 << 23);  // (256 rows within 32 bits)

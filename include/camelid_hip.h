@@ -452,7 +452,7 @@ int cml_dequantize_i8(const int8_t *q_dev, int64_t q_stride, const float *scales
  * 32-bit integer, the rest in f32, rounded once to dtype.  q int8[n_tokens][cols], w int8[rows][cols]
  * (any of the 256 values), bias_dev f32[rows] or null.  cols from 1 to 131071 (rows of no values are refused).  The bits depend neither on the
  * number of tokens nor on the kernel that serves the call.  Rows that start on 16-byte boundaries (base and stride, of q and
- * w both) run on the faster kernels. */
+ * w both; a single token's or row's stride does not count) run on the faster kernels. */
 int cml_matmul_i8(const int8_t *q_dev, int64_t q_stride, const float *scales_dev, int64_t n_tokens,
                   const int8_t *w_dev, int64_t w_stride, const float *w_scales_dev, int64_t rows,
                   int64_t cols, const float *bias_dev, int dtype, void *out_dev, int64_t out_stride,

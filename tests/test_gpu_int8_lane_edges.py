@@ -86,6 +86,29 @@ def test_very_long_rows_of_values_alike(t, cols, value):
     check_norm(t, bits, None, w, 1e-5, norm(t, bits, None, w, 1e-5))
 
 
+def strided_product(q, w, s, ws, bias, q_stride, w_stride):
+    B.init(0)
+    n, rows, cols = q.shape[0], w.shape[0], q.shape[1]
+    Q, W, O, S, WS, BI = Rows(q), Rows(w), Rows.empty(n, rows, np.uint32), f32(s), f32(ws), f32(bias)
+    G.say(f"matmul_i8 tokens={n} rows={rows} cols={cols} strides {q_stride} {w_stride}")
+    check(lib().cml_matmul_i8(Q.ptr, q_stride, S.ptr, n, W.ptr, w_stride, WS.ptr, rows, cols, BI.ptr, 0, O.ptr, rows, None))
+    check(lib().cml_stream_sync(None))
+    return O.get()
+
+
+@pytest.mark.parametrize("stride", [0, 1, 1025, -16, -1, (1 << 26) + 1, 1 << 40])
+def test_the_stride_of_a_single_row_says_nothing(stride):
+    q, w, s, ws, bias = operands(1, 1, 200, 1024)
+    with G.engaged("^i8.matmul.slim$", none=["any", "staged"]):
+        assert np.array_equal(strided_product(q, w, s, ws, bias, stride, 1024), want_product("f32", q, w, s, ws, bias))
+    q, w, s, ws, bias = operands(2, 40, 1, 1024)
+    with G.engaged("^i8.matmul.slim$", none=["any", "staged"]):
+        assert np.array_equal(strided_product(q, w, s, ws, bias, 1024, stride), want_product("f32", q, w, s, ws, bias))
+    q, w, s, ws, bias = operands(3, 1, 1, 1024)
+    with G.engaged("^i8.matmul.slim$", none=["any", "staged"]):
+        assert np.array_equal(strided_product(q, w, s, ws, bias, stride, stride), want_product("f32", q, w, s, ws, bias))
+
+
 def launched(call, name):
     before = G.launch_counts().get(name, 0)
     out = call()
