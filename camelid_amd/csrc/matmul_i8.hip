@@ -289,8 +289,9 @@ struct TileWork {
     __device__ __forceinline__ void touch(int step) {
         if constexpr (kTouch) {
             const int8_t *at = touched + step * KB;
-            asm volatile("s_mov_b32 m0, %0" ::"s"(__builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage + wave * 256)) : "memory", "m0");
-            if (touches) asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at) : "memory", "m0");
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage + wave * 256);
+            // (m0 is set where it is used: between two statements it could become another)
+            if (touches) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(at) : "memory", "m0");
         }
     }
     template <int SPLIT>
