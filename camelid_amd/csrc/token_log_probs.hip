@@ -136,14 +136,18 @@ __device__ __forceinline__ void close(RowState &s) {
     s.esum = wave_allsum(s.esum);
 }
 
+// The largest logit's own term is 2^shift, the same instruction's result as in the sums, and goes out of them before anything is rounded: S is the sum divided by it, 1 or more, and
+// what is left for the entropy is the other tokens'.  So no log probability is above 0 and no entropy below, and a row with one token left has 0 and 0.
 template <class T>
 __device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, const RowState &s, float given, bool in_range, int lane) {
-    const float all = __builtin_amdgcn_logf(s.sum), log_sum = (all - shift(s.most)) * kLn2;
+    const float more = shift(s.most), own = __builtin_amdgcn_exp2f(more);
+    const float all = __builtin_amdgcn_logf(s.sum / own), log_sum = all * kLn2;
+    const float entropy = (all - ((s.esum - own * more) - more * (s.sum - own)) / s.sum) * kLn2;
     const bool empty = s.sum == 0.0f;
     if (lane == 0) {
         a.log_prob[row] = !in_range ? __builtin_nanf("") : empty ? -INFINITY : (given - s.most) - log_sum;
         if (a.rank) a.rank[row] = in_range ? s.above + 1 : 0;
-        if (a.entropy) a.entropy[row] = empty ? 0.0f : (all - s.esum / s.sum) * kLn2;
+        if (a.entropy) a.entropy[row] = empty ? 0.0f : entropy;
     }
     if (lane < a.n_top) {
         a.top_ids[row * a.n_top + lane] = s.list ? static_cast<int>(~s.list_low) : -1;

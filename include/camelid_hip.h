@@ -478,6 +478,7 @@ int cml_moe_route_scored(int score, int dtype, const void *logits_dev, int64_t l
  * n_top (0 to 64) best tokens in order, ties to the lower index, with their log probabilities
  * (top_ids int32[n_rows*n_top], top_log_probs f32; null for n_top = 0).  Sums in f32, cut by n_rows and
  * vocab: the last bits may differ between calls of different n_rows, and with them only.
+ * No log probability is above 0 and no entropy below 0; a row with one token left has exactly 0 and 0.
  * -inf is a masked token: probability 0, never an alternative; slots without a token have id -1 and
  * -inf.  A row of masked tokens: log probability -inf, entropy 0.  A target outside the
  * vocabulary: log probability NaN, rank 0.  NaN or +inf in a row: NaN in log probabilities and entropy.
