@@ -109,6 +109,16 @@ def test_the_stride_of_a_single_row_says_nothing(stride):
         assert np.array_equal(strided_product(q, w, s, ws, bias, stride, stride), want_product("f32", q, w, s, ws, bias))
 
 
+@pytest.mark.parametrize("t,n,rows,out_pad", [("bf16", 3100, 16512, 0), ("bf16", 3100, 16513, 0), ("f32", 1700, 16384, 32), ("f32", 1700, 16384, 1)])
+def test_large_outputs_cell_by_cell(t, n, rows, out_pad):
+    q, w, s, ws, bias = operands(n, n, rows, 144)
+    with G.engaged("^i8.matmul.walk$"):
+        got = product(t, q, w, s, ws, bias, out_pad=out_pad)
+    for r in range(0, rows, 2048):
+        at = slice(r, r + 2048)
+        assert np.array_equal(got[:, at], want_product(t, q, w[at], s, ws[at], bias[at])), r
+
+
 def launched(call, name):
     before = G.launch_counts().get(name, 0)
     out = call()
