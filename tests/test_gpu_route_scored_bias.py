@@ -16,6 +16,20 @@ pytestmark = pytest.mark.gpu
 CASES = [(256, 8, 4, 2, 8), (160, 8, 3, 1, 6), (64, 16, 3, 2, 5), (60, 5, 2, 2, 7), (48, 48, 6, 2, 6), (64, 64, 64, 1, 64), (1024, 64, 9, 2, 20), (1024, 1, 1, 1, 16), (12, 1, 1, 2, 3), (320, 4, 4, 2, 16)]
 
 
+def inputs(experts, groups):
+    rng = np.random.default_rng(experts + groups)
+    return (rng.integers(-32, 32, (24, experts)) / 4.0).astype(np.float32), rng.uniform(-1, 1, experts).astype(np.float32)
+
+
+@pytest.mark.parametrize("quarter", [0, 1])
+@pytest.mark.parametrize("renormalise", [0, 1])
+@pytest.mark.parametrize("experts,groups,kept,group_top,k", CASES)
+def test_softmax_with_bias(experts, groups, kept, group_top, k, renormalise, quarter):
+    logits, bias = inputs(experts, groups)
+    with G.env(CAMELID_HIP_ROUTE_QUARTER=1 if quarter else 1 << 30):
+        compare(SOFTMAX, "f32", to_bits(logits, "f32"), bias, groups, kept, group_top, k, renormalise, 2.5, least=1.0)
+
+
 @pytest.mark.parametrize("quarter", [0, 1])
 def test_tokens_in_several_launches(quarter):
     B.init(0)
