@@ -50,11 +50,12 @@ __device__ __forceinline__ const int8_t *wave_uniform(const int8_t *p) {
 // are added up.  A request brings whole lines, eight to an instruction: what a unit takes in goes by the lines it has in flight, and in half lines, sixteen to an instruction, straight to
 // the lanes that multiply them, it is half as much.  Slot p of a row holds piece p ^ key(row), as below.
 //
-// 16 tokens on 4096 x 14336: 13.5 us (in half lines 18.5), on 352 x 15040 8.7 (21); 32 tokens on 4096 x 14336 16.6 (in tiles of 64 x 32 31.6), 64 on 1024 x 4096 4.8 (8.8).  What
-// bounds it is the weight's way from memory (4.9 TB/s of it at 4096 x 14336, one token) and for more tokens theirs from the L2.
+// Side by side: 16 tokens on 4096 x 14336 13.5 us (in half lines 18.5), on 352 x 15040 8.7 (21); 32 tokens on 4096 x 14336 16.6 (in tiles of 64 x 32 31.6), 64 on 1024 x 4096 4.8 (8.8).
+// 1 / 16 / 32 / 64 tokens on 4096 x 14336 with the weight in the last-level cache 11.6 / 12.1 / 12.8 / 15.3 us, from memory 13.8 / 15.0 / 18.1 / 21.7.  What bounds it is the weight's way
+// (one token 5.1 and 4.3 TB/s) and for more tokens theirs from the L2.
 //
-// ANY: rows that start anywhere.  Their lines pass through registers (which takes any address), two of them on their way.  Rows of 4099: one token on 4096 x 4099 5.8 us, 16 6.9;
-// in half lines 8.8 and 13.6.
+// ANY: rows that start anywhere.  Their lines pass through registers (which takes any address), two of them on their way.  Rows of 4099: one token on 4096 x 4099 5.8 us, 16 6.9,
+// in half lines 8.8 and 13.6 (one weight over and over; with three in turn 6.9 and 8.1).
 template <class T, int RT, int TT, int WAVES, int STAGES, bool ANY>
 __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) {
     constexpr int kRows = 16 * RT, kStage = 16 * (RT + TT) * 128, kFetches = 2 * (RT + TT);
@@ -184,8 +185,8 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_i8_slim_kernel(MatmulI8 a) 
 //
 // The instruction's 32 rows are the tile's in another order: a lane ends up with 16 neighbouring weight rows of its token and stores them whole.
 //
-// 37 tokens on 128256 x 2048: 50 us, the weight and the logits at 5.6 TB/s.  4096 x 14336 x 4096 (the walk): 222 us, 2.2 POPS; the matrix cores execute 56 % of the busy
-// cycles, LDS conflicts are gone, and the clock is the limit: under this load it falls from 2.4 to 1.8 GHz (8192 x 8192 x 8192: 451 us, of zeros 335).
+// 37 tokens on 128256 x 2048: 54 us, the weight and the logits at 5.2 TB/s.  4096 x 14336 x 4096 (the walk): 217 - 225 us, 2.2 POPS; the matrix cores execute 56 % of the busy
+// cycles, LDS conflicts are gone, and the clock is the limit: under this load it falls from 2.4 to 1.8 GHz (8192 x 8192 x 8192: 455 - 463 us, of zeros 335).
 typedef int v16i_i8 __attribute__((ext_vector_type(16)));
 
 struct TileGrid {
@@ -745,8 +746,10 @@ static int launch_walk(const MatmulI8 &a, hipStream_t st) {
 }
 
 // What a call takes by tile, in microseconds: a start, then per workgroup that a compute unit runs `work` for each step of 128 values and `ends` for the tile;
-// no tile is through its steps faster than `step` each, alone on its unit.  Fitted to 1 - 4096 tokens on weights from 64 x 512 to 128256 x 2048: the tile that it picks takes
-// 0.8 % more than the best one in the mean, 25 % at most.
+// no tile is through its steps faster than `step` each, alone on its unit.  Fitted to one weight over and over, 1 - 4096 tokens on 64 x 512 to 128256 x 2048, so that smaller ones were in the
+// caches; it has no term for memory.  With weights from memory (twelve shapes from 1024 x 4096 to 151936 x 1024, as many of each in turn as make 1.2 GB, 1 - 512 tokens) a call takes
+// 1.1 to 2.4 times what it says, and yet the order of the tiles holds: the one that is picked takes 1.4 % more than the best one in the mean, 15 % at most (16 tokens on 14336 x 4096: 16.7 us, in
+// tiles of 64 x 64 that ask for the weight past the caches 14.6); with small weights in the caches 1.8 % and 25 % (the same call: 14.8, in tiles of 64 x 32 11.9).
 struct TileCost {
     int rows, tokens, per_unit;
     float start, step, work, ends;
@@ -785,7 +788,8 @@ static int choose_aligned(const MatmulI8 &a) {
     const int64_t bytes = static_cast<int64_t>(a.rows) * a.cols;
     // A weight of 96 MB and more is used once in a pass over a model: past the caches (128256 x 2048, 1 / 16 / 37 tokens: 52 / 55 / 59 us plain, 45 / 46 / 49 so), in the
     // tile that has two workgroups for every compute unit (32000 x 4096, 1 / 32 tokens: 128 x 64 31 / 29, 64 x 64 29 / 28; 48 tokens: 30 / 30, plain 24), where that is a tile for every unit
-    // (4096 x 28672, one token: 62, plain and slim 25).
+    // (4096 x 28672, one token: 62, plain and slim 25).  With weights from memory, 1 and 64 tokens, 128 x 64 / 64 x 64 past the caches: 65536 x 2048 23.4 and 26.0 / 26.6 and 32.0 us,
+    // 151936 x 1024 32.7 and 39.8 / 33.3 and 43.7, 128256 x 2048 43.4 and 53.6 / 45.6 and 61.8; on 100352 x 4096 the smaller one is ahead, 81.4 and 93.2 / 74.2 and 91.1.
     if (bytes >= 96ll << 20 && a.n_tokens <= 64) {
         if ((a.rows + 127) / 128 >= 512) return 6;
         if (a.n_tokens <= 32 && (a.rows + 63) / 64 >= 256) return 7;

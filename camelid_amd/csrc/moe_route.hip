@@ -150,7 +150,7 @@ __device__ __forceinline__ int lanes_worth(const RouteArgs &a, const int (&rated
 }
 
 // A wave per token.  The logits are little to read; what it takes is instructions: a sigmoid's exponential and division are 25 for every expert, a turn of the
-// choice about 30, so that 8 of 256 for 8192 tokens (4 MB) come to 11.7 us, where reading them takes 1.  One token: 4.3 us, most of it the launch.
+// choice about 30, so that 8 of 256 for 8192 tokens (4 MB) come to 11.6 us, where reading them takes 1.  One token: 8 of 128 3.2 us, most of it the launch, 8 of 256 in 8 groups 4.3.
 template <class T, bool SIGMOID, int NE>
 __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -214,8 +214,8 @@ __global__ __launch_bounds__(256) void moe_route_scored_kernel(RouteArgs a) {
 // Four tokens a wave, 16 lanes each, for up to MOST of 16 * NE experts.  Every lane sorts its experts first, as doubles: a value's f32 bits are the upper word (finite
 // and infinite floats are finite doubles, in the same order), its place the lower one, so that a comparison that the chip makes at full rate decides ties as well.
 // Then the lanes' first entries meet k times, and the lane that held the best goes on to its next.  A turn's
-// maximum over 16 lanes serves four tokens, so a token takes 340 instructions in place of some 600: 8 of 256 for 8192 tokens 8.4 us, two waves to a SIMD and bound by the
-// latency of their chains.
+// maximum over 16 lanes serves four tokens, so a token takes 340 instructions in place of some 600: 8 of 256 for 8192 tokens 8.1 us, two waves to a SIMD and bound by the
+// latency of their chains; 16 of 512 15.0 us, 680 instructions, which issue in two thirds of the busy cycles.
 __device__ __forceinline__ void sort_two(double &a, double &b) {  // descending
     const double hi = __builtin_fmax(a, b);
     b = __builtin_fmin(a, b);
@@ -356,8 +356,8 @@ static int launch_route(RouteArgs a, hipStream_t st) {
     while (a.n_groups << (a.group_shift + 1) <= 64 && (a.group_shift < 4 || a.n_groups == 1)) a.group_shift++;
     int ne = 1;
     while (ne << a.group_shift < a.group_size) ne *= 2;
-    // Four tokens a wave where there are waves enough that way (8 of 256 in 8 groups, four against one: 1024 tokens 6.3 and 4.9 us, 4096 6.9 and 7.7, 8192 8.4
-    // and 11.7; 16 of 512, 8192 tokens: 19.1 and 22.8).
+    // Four tokens a wave where there are waves enough that way (8 of 256 in 8 groups, four against one: 1024 tokens 6.6 and 5.3 us, 4096 6.7 and 7.5, 8192 8.1
+    // and 11.6; 16 of 512, 8192 tokens: 15.0 and 21.0).
     if (a.n_tokens >= env_int("CAMELID_HIP_ROUTE_QUARTER", 4096) && a.k <= 16 && a.group_shift >= 2 && ne <= 8) {
         a.group_shift -= 2;
         return a.k <= 8 ? launch_route_quarters<T, SIGMOID, 8>(a, 4 * ne, st) : launch_route_quarters<T, SIGMOID, 16>(a, 4 * ne, st);

@@ -10,8 +10,8 @@
 // Logits are looked at one by one for the list only where a batch holds one above the list's last.  Where it holds many (the first one; ascending
 // logits), a bisection over the lanes' maxima first finds a value that at least n of the batch reach, and one over all its logits where that leaves too many.
 //
-// Rows are to be read once, at memory's rate: 2048 x 128256 bf16 in 95 us without a list (5.5 TB/s), 113 with 20 best; what bounds the latter is instruction issue, 12
-// to a logit and 80 insertions a part.  One row of 128256 f32 and 20 best: 10.9 us, two launches of which each waits for memory once.
+// Rows are to be read once, at memory's rate: 2048 x 128256 bf16 in 94 us without a list (5.6 TB/s), 114 with 20 best; what bounds the latter is instruction issue, 11
+// to a logit and 80 insertions a part.  With fewer rows the lists weigh more, since every part fills one of its own: 512 rows 32 us without a list (4.1 TB/s), 35 with one best, 39 with 5, 50 with 20.  One row of 128256 f32 and 20 best: 11.0 us, two launches of which each waits for memory once.
 //
 // -inf is a masked token: probability 0, no alternative.  A row of nothing else has log probability -inf, entropy 0 and no alternatives.  NaN or +inf in a
 // row leaves NaN in log probability and entropy, as the formula does.  A row at the type's lowest value is an ordinary, uniform row.
